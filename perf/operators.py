@@ -1,0 +1,369 @@
+"""The operators around the 4-bit linears of the DiT blocks, as cases to measure.
+
+  quantise   rows of activations -> MXFP4 (OCP microscaling: 32 consecutive e2m1 values share one power-of-two scale) and back
+  linear     C = epilogue(mxfp4(x) W^T) on weights held in MXFP4
+  norm       the residual update that ends one half of a block and the norm that opens the next half, in one pass over the stream:
+             x' = x + gate * [norm](y + bias) + offset,  h = norm(x') * w + b, * (1 + scale) + shift
+  ffn        the three together as a block runs them: norm -> linear + GELU -> linear, MXFP4 between all of them
+
+`own` False: plain torch, in 32 bits.  `own` True: the calls of fantasy_world_amd.hip_ops.HipOps.
+
+MXFP4 as used here: the scale byte of a block is the exponent of its largest magnitude minus 2, one more where that magnitude has a
+mantissa of 1.75 or above (it would round past 6, the largest e2m1 value), and never below 0 (2^-127); values round to the nearest, ties to
+the even code.  Rows are packed two values a byte, the first in the low half, and padded with zeros to a multiple of 256 values; scale bytes
+lie as [rows / 32][K / 256][32][8]: the 8 scales that a row needs for 256 values next to those of its 31 neighbours.
+"""
+import torch
+
+own = False
+
+DEV = "cuda"
+_ops = None
+
+
+def listed():
+    return [
+        # one token's row, as the first thing a single-token linear does: latency
+        dict(name="quantise 1x5120", op="quantise", M=1, K=5120, strided=False),
+        # the FFN's hidden rows of a 81-frame 480p video: the largest activation that is ever quantised
+        dict(name="quantise 32760x13824", op="quantise", M=32760, K=13824, strided=False),
+        # a single token through a square projection: the weights are all there is to read
+        dict(name="linear 1x5120x5120", op="linear", M=1, N=5120, K=5120, act="none", gate=False, res="none", out="bf16", strided=False),
+        # the 21 camera tokens of a video through an MLP's first layer
+        dict(name="linear 21x4096x1024", op="linear", M=21, N=4096, K=1024, act="gelu_erf", gate=False, res="none", out="bf16", strided=False),
+        # 512 text tokens -> keys and values of a cross-attention
+        dict(name="linear 512x10240x5120", op="linear", M=512, N=10240, K=5120, act="none", gate=False, res="none", out="bf16", strided=False),
+        # one frame's tokens with its five special ones, back onto the fp32 stream with a gate
+        dict(name="linear 1565x5120x13824", op="linear", M=1565, N=5120, K=13824, act="none", gate=True, res="f32", out="f32", strided=False),
+        # the fused q | k | v projection of a whole 81-frame 480p video: the largest product of a step
+        dict(name="linear 32760x15360x5120", op="linear", M=32760, N=15360, K=5120, act="none", gate=False, res="none", out="bf16", strided=True),
+        # a single row of the stream: latency
+        dict(name="norm 1x5120", op="norm", M=1, C=5120, x="f32", y="bf16", post="none", norm="layer", affine=False, mod=True, groups=1),
+        # the DiT stream of a video behind an all-reduced projection, into the modulated norm of the next half
+        dict(name="norm 32760x5120", op="norm", M=32760, C=5120, x="f32", y="bf16", post="none", norm="layer", affine=False, mod=True, groups=1),
+        # a narrow stream held in bf16 with norms on both sides of the block, two samples with modulations of their own
+        dict(name="norm 8190x1024", op="norm", M=8190, C=1024, x="bf16", y="f32", post="rms", norm="rms", affine=True, mod=True, groups=2),
+        # the FFN half of a block for the image tokens of one prompt
+        dict(name="ffn 257x5120x13824", op="ffn", M=257, C=5120, F=13824),
+        # the same for a 21-frame video at a quarter of the 480p grid
+        dict(name="ffn 8190x5120x13824", op="ffn", M=8190, C=5120, F=13824),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(lo * (hi / lo) ** rng.random()))
+
+
+def _size(rng, lo, hi):
+    n = _log(rng, lo, hi)
+    return min(hi, -(-n // 64) * 64) if rng.random() < 0.5 else n
+
+
+def draw(rng):
+    op = rng.choice(["quantise", "linear", "linear", "norm", "norm", "ffn"])
+    if op == "quantise":
+        return dict(op=op, M=_log(rng, 1, 32760), K=_size(rng, 32, 13824), strided=rng.random() < 0.5)
+    if op == "linear":
+        res = rng.choice(["none", "none", "bf16", "f32"])
+        return dict(op=op, M=_log(rng, 1, 32760), N=_size(rng, 64, 15360), K=_size(rng, 64, 5120),
+                    act=rng.choice(["none", "none", "relu", "gelu_tanh", "gelu_erf", "silu"]), gate=rng.random() < 0.5, res=res,
+                    out="f32" if res == "f32" else "bf16", strided=rng.random() < 0.5)
+    if op == "norm":
+        groups = rng.choice([1, 1, 2, 3])
+        return dict(op=op, M=groups * _log(rng, 1, 32760 // groups), C=_size(rng, 64, 5120), x=rng.choice(["f32", "bf16"]),
+                    y=rng.choice(["bf16", "f32", "none"]), post=rng.choice(["none", "none", "rms", "layer"]), norm=rng.choice(["layer", "layer", "rms"]),
+                    affine=rng.random() < 0.5, mod=rng.random() < 0.7, groups=groups)
+    return dict(op=op, M=_log(rng, 1, 8190), C=_size(rng, 64, 5120), F=_size(rng, 64, 13824))
+
+
+# ---- inputs ---------------------------------------------------------------------------------------------------------------------------
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(int(seed))
+
+
+def _acts(g, rows, cols, dtype=torch.bfloat16, strided=False):
+    """Activations as they leave a modulated norm: a gain of its own for every channel, and a few channels far above the rest."""
+    gain = torch.exp(0.5 * torch.randn(cols, generator=g, device=DEV))
+    gain = gain * torch.where(torch.rand(cols, generator=g, device=DEV) < 0.005, 12.0, 1.0)
+    wide = torch.empty(rows, cols + 64 if strided else cols, dtype=dtype, device=DEV)      # strided: columns of a wider projection
+    out = wide[:, :cols]
+    for a in range(0, rows, 4096):
+        out[a:a + 4096] = torch.randn(min(4096, rows - a), cols, generator=g, device=DEV) * gain
+    return out
+
+
+def _vec(g, n, scale=0.1):
+    return torch.randn(n, generator=g, device=DEV) * scale
+
+
+def _weights(g, N, K):
+    """A linear's weights as a program keeps them: packed codes, scale bytes in the order above, bias."""
+    w = torch.randn(N, K, generator=g, device=DEV) * K ** -0.5
+    code, byte = _codes(w)
+    q = (code[:, 0::2] | (code[:, 1::2] << 4)).contiguous()
+    rows = -(-N // 32) * 32
+    s = torch.zeros(rows, byte.shape[1], dtype=torch.uint8, device=DEV)
+    s[:N] = byte
+    return dict(q=q, s=s.view(rows // 32, 32, -1, 8).permute(0, 2, 1, 3).contiguous(), b=_vec(g, N), N=N, K=K)
+
+
+def prepare(case, seed):
+    g, op = _gen(seed), case["op"]
+    st = dict(case=case)
+    if op == "quantise":
+        st["x"] = _acts(g, case["M"], case["K"], strided=case["strided"])
+    elif op == "linear":
+        M, N = case["M"], case["N"]
+        st["x"] = _acts(g, M, case["K"], strided=case["strided"])
+        st["w"] = _weights(g, N, case["K"])
+        st["g1"] = _vec(g, N, 0.5) if case["gate"] else None
+        st["res"] = None if case["res"] == "none" else _acts(g, M, N, torch.float32 if case["res"] == "f32" else torch.bfloat16)
+    elif op == "norm":
+        M, C, n = case["M"], case["C"], case["groups"]
+        dt = dict(f32=torch.float32, bf16=torch.bfloat16)
+        st["x"] = _acts(g, M, C, dt[case["x"]])
+        st["y"] = None if case["y"] == "none" else _acts(g, M, C, dt[case["y"]])
+        st["bias"], st["g1"], st["g0"] = _vec(g, C), _vec(g, n * C, 0.5).view(n, C), _vec(g, n * C).view(n, C)
+        st["post_w"] = 1 + _vec(g, C)
+        st["w"], st["b"] = (1 + _vec(g, C), _vec(g, C)) if case["affine"] else (None, None)
+        st["scale"], st["shift"] = (_vec(g, n * C).view(n, C), _vec(g, n * C).view(n, C)) if case["mod"] else (None, None)
+        st["x_out"] = torch.empty_like(st["x"])
+    else:
+        M, C, F = case["M"], case["C"], case["F"]
+        st["x"], st["y"] = _acts(g, M, C, torch.float32), _acts(g, M, C)
+        st["bias"], st["g1"] = _vec(g, C), _vec(g, C, 0.5)
+        st["scale"], st["shift"] = _vec(g, C), _vec(g, C)
+        st["w0"], st["w2"] = _weights(g, F, C), _weights(g, C, F)
+        st["x_out"] = torch.empty_like(st["x"])
+    return st
+
+
+# ---- the plain forms ------------------------------------------------------------------------------------------------------------------
+
+
+def _codes(x):
+    """e2m1 codes (uint8, one a value) and scale bytes of the rows of x, both padded to whole groups of 256 values."""
+    rows, K = x.shape
+    v = torch.nn.functional.pad(x.float(), (0, -K % 256)).view(rows, -1, 32)
+    top = v.abs().amax(2).view(torch.int32)
+    byte = ((top >> 23) - 2 + ((top & 0x7fffff) >= 0x600000)).clamp(min=0)
+    byte = torch.where((top >> 23) == 255, 255, byte)                     # infinities and NaN: the scale is NaN
+    a = v.abs().double() * torch.exp2(127.0 - byte.double()).unsqueeze(2)
+    code = (a > 0.25).byte() + (a >= 0.75).byte() + (a > 1.25).byte() + (a >= 1.75).byte() + (a > 2.5).byte() + (a >= 3.5).byte() + (a > 5).byte()
+    code += 8 * torch.signbit(v).byte()
+    return code.view(rows, -1), byte.to(torch.uint8)
+
+
+def _values(code, byte, K):
+    """What codes and scale bytes stand for, in 32 bits."""
+    level = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.0, -0.5, -1, -1.5, -2, -3, -4, -6], device=code.device)
+    scale = torch.where(byte == 255, torch.nan, torch.exp2(byte.double() - 127)).float()
+    v = level[code.int()].view(code.shape[0], -1, 32) * scale.unsqueeze(2)
+    return v.view(code.shape[0], -1)[:, :K]
+
+
+def _rounded(x):
+    return _values(*_codes(x), x.shape[1])
+
+
+def _unpacked(w):
+    q, s, N = w["q"], w["s"], w["N"]
+    code = torch.stack([q & 15, q >> 4], dim=2).view(N, -1)
+    return _values(code, s.permute(0, 2, 1, 3).reshape(-1, code.shape[1] // 32)[:N], w["K"])
+
+
+def _act(v, act):
+    if act == "relu":
+        return v.clamp(min=0)
+    if act == "gelu_tanh":
+        return 0.5 * v * (1 + torch.tanh(0.7978845608028654 * (v + 0.044715 * v * v * v)))
+    if act == "gelu_erf":
+        return 0.5 * v * (1 + torch.erf(v * 0.7071067811865476))
+    if act == "silu":
+        return v / (1 + torch.exp(-v))
+    return v
+
+
+def _linear(x, w, act="none", g1=None, res=None):
+    v = _act(_rounded(x) @ _unpacked(w).t() + w["b"], act)
+    if g1 is not None:
+        v = v * g1
+    return v if res is None else v + res.float()
+
+
+def _normed(v, kind, eps=1e-6):
+    if kind == "layer":
+        v = v - v.mean(1, keepdim=True)
+    return v * torch.rsqrt((v * v).mean(1, keepdim=True) + eps)
+
+
+def _by_group(v, rows):
+    return v if v is None or v.dim() == 1 or v.shape[0] == 1 else v.repeat_interleave(rows // v.shape[0], 0)
+
+
+def _residual_norm(x, y, bias, g1, g0, post, post_w, w, b, scale, shift, norm):
+    rows, dt = x.shape[0], x.dtype
+    x = x.float()
+    if y is not None:
+        t = y.float() + bias
+        if post != "none":
+            t = _normed(t, post) * post_w
+        t = t * _by_group(g1, rows)
+        x = x + (t if g0 is None else t + _by_group(g0, rows))
+    x = x.to(dt)
+    h = _normed(x.float(), norm)
+    if w is not None:
+        h = h * w + b
+    if scale is not None:
+        h = h * (1 + _by_group(scale, rows)) + _by_group(shift, rows)
+    return x, h.bfloat16()
+
+
+# ---- one pass -------------------------------------------------------------------------------------------------------------------------
+
+
+def _hip():
+    global _ops
+    if _ops is None:
+        from fantasy_world_amd.hip_ops import HipOps
+        _ops = HipOps(DEV)
+    return _ops
+
+
+def _packed(w):
+    return _hip().linear_from_mxfp4(w["q"], w["s"], w["b"], w["K"])
+
+
+def run(st):
+    c = st["case"]
+    op = c["op"]
+    if op == "quantise":
+        if own:
+            ops = _hip()
+            return ops.dequantize_mxfp4_rows(ops.quantize_mxfp4_rows(st["x"]))
+        return _rounded(st["x"]).bfloat16()
+    if op == "linear":
+        if own:
+            return _hip().linear(st["x"], _packed(st["w"]), act=c["act"], g1=st["g1"], res=st["res"], out_f32=c["out"] == "f32")
+        v = _linear(st["x"], st["w"], c["act"], st["g1"], st["res"])
+        return v if c["out"] == "f32" else v.bfloat16()
+    if op == "norm":
+        if own:
+            h = _hip().residual_norm(st["x"], st["y"], bias=st["bias"], g1=st["g1"], g0=st["g0"], post=c["post"], post_w=st["post_w"], w=st["w"],
+                                     b=st["b"], scale=st["scale"], shift=st["shift"], norm=c["norm"], eps=1e-6, x_out=st["x_out"])
+            return dict(h=h) if c["y"] == "none" else dict(x=st["x_out"], h=h)
+        x, h = _residual_norm(st["x"], st["y"], st["bias"], st["g1"], st["g0"], c["post"], st["post_w"], st["w"], st["b"], st["scale"],
+                              st["shift"], c["norm"])
+        return dict(h=h) if c["y"] == "none" else dict(x=x, h=h)
+    if own:
+        ops = _hip()
+        h = ops.residual_norm(st["x"], st["y"], bias=st["bias"], g1=st["g1"], scale=st["scale"], shift=st["shift"], eps=1e-6, x_out=st["x_out"],
+                              out="mxfp4")
+        f = ops.linear(h, _packed(st["w0"]), act="gelu_tanh", out_mxfp4=True)
+        return dict(x=st["x_out"], out=ops.linear(f, _packed(st["w2"])))
+    x, h = _residual_norm(st["x"], st["y"], st["bias"], st["g1"], None, "none", None, None, None, st["scale"], st["shift"], "layer")
+    f = _linear(h, st["w0"], "gelu_tanh").bfloat16()
+    return dict(x=x, out=_linear(f, st["w2"]).bfloat16())
+
+
+# ---- what a pass cannot do without ----------------------------------------------------------------------------------------------------
+
+
+def work(case):
+    op, M = case["op"], case["M"]
+    size = dict(f32=4, bf16=2, none=0)
+    held = 0.5 + 1 / 32                                                  # bytes of an MXFP4 value
+    if op == "quantise":
+        n = M * case["K"]
+        return dict(bytes=n * (2 + held + 2), flops=4 * n)
+    if op == "linear":
+        N, K = case["N"], case["K"]
+        b = M * K * 2 + N * K * held + N * 4 * (2 if case["gate"] else 1) + M * N * (size[case["res"]] + size[case["out"]])
+        return dict(bytes=b, flops=2 * M * N * K)
+    if op == "norm":
+        n = M * case["C"]
+        b = n * (size[case["x"]] * (1 if case["y"] == "none" else 2) + size[case["y"]] + 2)
+        return dict(bytes=b, flops=12 * n)
+    C, F = case["C"], case["F"]
+    return dict(bytes=M * C * (4 + 4 + 2 + 2) + 2 * C * F * held, flops=4 * M * C * F)
+
+
+# ---- the definition, in 64 bits -------------------------------------------------------------------------------------------------------
+
+
+def _round64(x):
+    """MXFP4 of rows in 64 bits: the step between neighbouring e2m1 values is a half below 2, one below 4, two above."""
+    out = torch.empty(x.shape, dtype=torch.float64, device=x.device)
+    for k in range(0, x.shape[1], 32):
+        v = x[:, k:k + 32].double()
+        m, e = torch.frexp(v.abs().amax(1, keepdim=True))                # m in [1/2, 1)
+        unit = torch.ldexp(torch.ones_like(m), (e - 3 + (m >= 0.875)).clamp(min=-127))
+        a = v / unit
+        step = torch.where(a.abs() < 2, 0.5, torch.where(a.abs() < 4, 1.0, 2.0))
+        out[:, k:k + 32] = (torch.round(a / step) * step).clamp(-6, 6) * unit
+    return out
+
+
+def _weights64(w):
+    N, K = w["N"], w["K"]
+    byte = torch.cat(list(w["s"].unbind(1)), dim=2).reshape(-1, w["q"].shape[1] // 16)[:N]
+    half = torch.tensor([0, 1, 2, 3, 4, 6, 8, 12], dtype=torch.float64, device=DEV) / 2
+    out = torch.empty(N, w["q"].shape[1] * 2, dtype=torch.float64, device=DEV)
+    for first, code in ((0, w["q"] % 16), (1, w["q"] // 16)):
+        out[:, first::2] = half[(code % 8).long()] * torch.where(code >= 8, -1.0, 1.0).double()
+    return (out * torch.pow(2.0, byte.double() - 127).repeat_interleave(32, 1))[:, :K]
+
+
+def _act64(v, act):
+    if act == "relu":
+        return torch.maximum(v, torch.zeros_like(v))
+    if act == "gelu_tanh":
+        return v * torch.sigmoid((v + 0.044715 * v.pow(3)) * (2 * (2 / torch.pi) ** 0.5))
+    if act == "gelu_erf":
+        return v * 0.5 * torch.special.erfc(-v / 2 ** 0.5)
+    return v * torch.sigmoid(v) if act == "silu" else v
+
+
+def _linear64(x, w, act="none"):
+    return _act64(_round64(x) @ _weights64(w).t() + w["b"].double(), act)
+
+
+def _norm64(v, kind):
+    if kind == "layer":
+        return (v - v.mean(1, keepdim=True)) / (v.var(1, unbiased=False, keepdim=True) + 1e-6).sqrt()
+    return v / (v.square().mean(1, keepdim=True) + 1e-6).sqrt()
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    op = case["op"]
+    if op == "quantise":
+        return _round64(st["x"])
+    if op == "linear":
+        v = _linear64(st["x"], st["w"], case["act"])
+        if st["g1"] is not None:
+            v *= st["g1"].double()
+        if st["res"] is not None:
+            v += st["res"].double()
+        return v
+    rows = st["x"].shape[0]
+    each = (lambda v: v.double().view(-1, 1, v.shape[-1]).expand(-1, rows // max(1, v.numel() // v.shape[-1]), -1).reshape(rows, -1))
+    x = st["x"].double()
+    if st["y"] is not None:
+        t = st["y"].double() + st["bias"].double()
+        if op == "norm" and case["post"] != "none":
+            t = _norm64(t, case["post"]) * st["post_w"].double()
+        t = t * each(st["g1"])
+        x = x + (t + each(st["g0"]) if op == "norm" else t)
+    kept = x.to(st["x"].dtype).double()                                  # the norm reads the stream as it is stored
+    h = _norm64(kept, case["norm"] if op == "norm" else "layer")
+    if op == "norm" and st["w"] is not None:
+        h = h * st["w"].double() + st["b"].double()
+    if st["scale"] is not None:
+        h = h * (1 + each(st["scale"])) + each(st["shift"])
+    if op == "norm":
+        return dict(h=h) if st["y"] is None else dict(x=x, h=h)
+    f = _linear64(h.bfloat16(), st["w0"], "gelu_tanh")
+    return dict(x=x, out=_linear64(f.bfloat16(), st["w2"]))
