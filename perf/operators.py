@@ -299,7 +299,7 @@ def _round64(x):
     for k in range(0, x.shape[1], 32):
         v = x[:, k:k + 32].double()
         m, e = torch.frexp(v.abs().amax(1, keepdim=True))                # m in [1/2, 1)
-        unit = torch.ldexp(torch.ones_like(m), (e - 3 + (m >= 0.875)).clamp(-127, 125))
+        unit = torch.exp2((e - 3 + (m >= 0.875)).clamp(-127, 125).double())      # exact: pow(2, n) is not, on a GPU
         a = v / unit
         step = torch.where(a.abs() < 2, 0.5, torch.where(a.abs() < 4, 1.0, 2.0))
         out[:, k:k + 32] = (torch.round(a / step) * step).clamp(-6, 6) * unit
@@ -313,7 +313,7 @@ def _weights64(w):
     out = torch.empty(N, w["q"].shape[1] * 2, dtype=torch.float64, device=DEV)
     for first, code in ((0, w["q"] % 16), (1, w["q"] // 16)):
         out[:, first::2] = half[(code % 8).long()] * torch.where(code >= 8, -1.0, 1.0).double()
-    return (out * torch.pow(2.0, byte.double() - 127).repeat_interleave(32, 1))[:, :K]
+    return (out * torch.exp2(byte.double() - 127).repeat_interleave(32, 1))[:, :K]
 
 
 def _act64(v, act):
