@@ -23,15 +23,16 @@ flags=(--offload-arch=gfx950 "${nopk[@]}" -O3 -std=c++17 -fPIC -ffast-math -fno-
 objs=()
 pids=()
 names=()
-for f in gemm.hip gemm_pp.hip attention.hip elementwise.hip heads.hip fp8.hip gemm_fp8.hip attention_fp8.hip; do
+for f in gemm.hip gemm_pp.hip attention.hip elementwise.hip heads.hip fp8.hip gemm_fp8.hip attention_fp8.hip mxfp4.hip gemm_mxfp4.hip residual_norm.hip; do
   o="${here}/${f%.hip}${tag}.o"
   # rebuild decision by CONTENT, not by mtime (round 5: this container's clock stepped backwards by minutes mid-session, so edited
   # sources were "older" than their objects and a renamed kernel silently kept its old object): hash of source + headers + this script
-  want="$(cat "${here}/$f" "${here}/fw_common.h" "${here}/gemm_common.h" "${here}/../../include/fw_mi355x.h" "${BASH_SOURCE[0]}" | sha256sum | cut -d' ' -f1) ${FW_ATTN_EXTRA_FLAGS-default} ${FW_MFMA_EXTRA_FLAGS-}"
+  mine="$(grep -q '"mxfp4.h"' "${here}/$f" && echo "${here}/mxfp4.h"; grep -q '"row_norm.h"' "${here}/$f" && echo "${here}/row_norm.h"; true)"
+  want="$(cat "${here}/$f" "${here}/fw_common.h" "${here}/gemm_common.h" ${mine} "${here}/../../include/fw_mi355x.h" "${BASH_SOURCE[0]}" | sha256sum | cut -d' ' -f1) ${FW_ATTN_EXTRA_FLAGS-default} ${FW_MFMA_EXTRA_FLAGS-}"
   if [ ! -f "$o" ] || [ ! -f "$o.sha" ] || [ "$(cat "$o.sha")" != "$want" ]; then
     rm -f "$o" "$o.sha"
     echo "$want" > "$o.sha.new"
-    if [ "$f" = "fp8.hip" ] || [ "$f" = "elementwise.hip" ] || [ "$f" = "heads.hip" ]; then
+    if [ "$f" = "fp8.hip" ] || [ "$f" = "elementwise.hip" ] || [ "$f" = "heads.hip" ] || [ "$f" = "mxfp4.hip" ] || [ "$f" = "residual_norm.hip" ]; then
       # no -ffast-math: IEEE division for the fp8 quantiser; and (round 5) the row passes -- LayerNorm / RMSNorm statistics, RoPE,
       # GroupNorm, the head activations -- are HBM-bound, so the flag bought nothing there while it let the compiler re-associate
       # sums and replace divisions / rsqrt by approximations from one hipcc to the next (round 4 had to pin the LayerNorm statistics by

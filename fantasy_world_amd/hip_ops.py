@@ -14,9 +14,10 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # FW_LIB_PATH: A/B knob for kernel experiments (two builds of the library measured on one box); never a fallback
 LIB_PATH = os.environ.get("FW_LIB_PATH") or os.path.join(_HERE, "libfw_mi355x.so")
 
-FW_DT_NONE, FW_DT_BF16, FW_DT_F32 = 0, 1, 2
+FW_DT_NONE, FW_DT_BF16, FW_DT_F32, FW_DT_MXFP4 = 0, 1, 2, 3
 ACT = {None: 0, "none": 0, "relu": 1, "gelu_tanh": 2, "gelu_erf": 3, "silu": 4}
 NORM = {None: 0, "none": 0, "rms_full": 1, "ln_head": 2}
+RNORM = {None: 0, "none": 0, "layer": 1, "rms": 2}
 ROPE = {None: 0, "none": 0, "interleaved": 1, "half2d": 2}
 
 # every symbol declared in include/fw_mi355x.h (tests check the library exports all of them)
@@ -31,6 +32,7 @@ SYMBOLS = [
     "fw_row_sumsq", "fw_qk_prep_tp", "fw_residual_add", "fw_cfg_euler_step",
     "fw_qk_prep_fp8", "fw_v_transpose_e4m3", "fw_row_absmax", "fw_fp8_quant_rows_amax", "fw_modulation_tables",
     "fw_layernorm_mod_split",
+    "fw_mxfp4_quant_rows", "fw_mxfp4_dequant_rows", "fw_gemm_mxfp4", "fw_residual_norm",
 ]
 
 _lib = None
@@ -100,6 +102,10 @@ def load_library(path: str = LIB_PATH, cache: bool = True):
         "fw_fp8_quant_rows_amax": [vp, i64, vp, i64, vp, vp, i32, i32, vp],
         "fw_modulation_tables": [vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, vp],
         "fw_layernorm_mod_split": [vp, i64, vp, vp, i64, i32, i32, vp, vp, vp, vp, f32, vp],
+        "fw_mxfp4_quant_rows": [vp, i64, i32, vp, i64, vp, i32, i32, vp],
+        "fw_mxfp4_dequant_rows": [vp, i64, vp, vp, i64, i32, i32, i32, vp],
+        "fw_gemm_mxfp4": [vp, i64, vp, vp, i64, vp, vp, i64, i32, vp, i32, i32, i32, vp, i32, vp, vp, vp, i64, i32, vp],
+        "fw_residual_norm": [vp, i64, vp, i64, i32, vp, i64, i32, vp, vp, vp, i32, vp, i32, vp, vp, vp, vp, f32, vp, i64, i32, vp, i32, i32, i32, vp],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)
@@ -137,10 +143,49 @@ class Linear:
     fp8 = True: the weight is e4m3 bytes (raw cast) and the bias holds bf16-rounded values -- AutoWrappedLinear.fp8_linear's
     operands (diffsynth_wan22/vram_management/layers.py:134-138); HipOps.linear then quantises the activation rows."""
     __slots__ = ("w", "b", "N", "K", "fp8")
+    mxfp4 = False
 
     def __init__(self, w, b, fp8=False):
         self.w, self.b, self.fp8 = w, b, fp8
         self.N, self.K = w.shape
+
+
+class MXFP4Rows:
+    """A matrix held as MXFP4 rows (include/fw_mi355x.h): codes q uint8 [M, Kp / 2], scales s uint8 [ceil(M / 32), Kp / 256, 32, 8], Kp = K rounded
+    up to 256."""
+    __slots__ = ("q", "s", "M", "K")
+
+    def __init__(self, q, s, K):
+        if q.dtype != torch.uint8 or q.dim() != 2 or q.stride(1) != 1 or K <= 0 or q.shape[1] != (K + 255) // 256 * 128:
+            raise ValueError(f"MXFP4 codes: uint8 [M, roundup(K, 256) / 2] with contiguous rows expected, got {q.dtype} {tuple(q.shape)} for K = {K}")
+        want = ((q.shape[0] + 31) // 32, q.shape[1] // 128, 32, 8)
+        if s.dtype != torch.uint8 or tuple(s.shape) != want or not s.is_contiguous():
+            raise ValueError(f"MXFP4 scales: contiguous uint8 {want} expected, got {s.dtype} {tuple(s.shape)}")
+        if q.device != s.device:
+            raise ValueError(f"MXFP4 codes on {q.device}, scales on {s.device}")
+        self.q, self.s, self.M, self.K = q, s, q.shape[0], K
+
+    @property
+    def shape(self):
+        return (self.M, self.K)
+
+
+class LinearMXFP4(MXFP4Rows):
+    """Pre-packed nn.Linear with MXFP4 weights [N, K] and an fp32 bias [N]; HipOps.linear quantises the activation rows (or takes them as
+    MXFP4Rows)."""
+    __slots__ = ("b",)
+    fp8 = False
+    mxfp4 = True
+
+    def __init__(self, q, s, b, K):
+        super().__init__(q, s, K)
+        if b is not None and (b.dtype != torch.float32 or b.shape != (self.M,) or not b.is_contiguous()):
+            raise ValueError(f"bias: contiguous fp32 [{self.M}] expected, got {b.dtype} {tuple(b.shape)}")
+        self.b = b
+
+    @property
+    def N(self):
+        return self.M
 
 
 class LinearF32:
@@ -230,10 +275,12 @@ class HipOps:
     def to_act(self, t):
         return t.detach().to(device=self.device, dtype=torch.bfloat16).contiguous()
 
-    def pack_linear(self, w, b, fp8=False):
-        """w fp32/bf16 [N, K] with K % 64 == 0 (engine pads), b [N] or None.  fp8: pack for the fp8 linear instead."""
+    def pack_linear(self, w, b, fp8=False, mxfp4=False):
+        """w fp32/bf16 [N, K] with K % 64 == 0 (engine pads), b [N] or None.  fp8 / mxfp4: pack for the fp8 / MXFP4 linear instead."""
         if fp8:
             return self.pack_linear_fp8(w, b)
+        if mxfp4:
+            return self.pack_linear_mxfp4(w, b)
         assert w.shape[1] % 64 == 0, w.shape
         wb = w.detach().to(device=self.device, dtype=torch.bfloat16).contiguous()
         bb = None if b is None else b.detach().to(device=self.device, dtype=torch.float32).contiguous()
@@ -243,7 +290,12 @@ class HipOps:
         return LinearF32(self.to_f32(w), None if b is None else self.to_f32(b))
 
     # ---- GEMM -------------------------------------------------------------------------------------------------
-    def linear(self, x, lin, act=None, g1=None, g0=None, res=None, out_f32=False, out=None):
+    def linear(self, x, lin, act=None, g1=None, g0=None, res=None, out_f32=False, out=None, out_mxfp4=False):
+        """out_mxfp4 (MXFP4 linears): the result as MXFP4Rows, the input of the next MXFP4 linear."""
+        if lin.mxfp4:
+            return self._linear_mxfp4(x, lin, act, g1, g0, res, out_f32, out, out_mxfp4)
+        if out_mxfp4 or isinstance(x, MXFP4Rows):
+            raise ValueError("MXFP4 rows in or out need a linear packed with pack_linear_mxfp4 / linear_from_mxfp4")
         self._check_dev(x if not isinstance(x, tuple) else x[0], res, out, g1, g0)
         if lin.fp8:
             return self._linear_fp8(x, lin, act, g1, g0, res, out_f32, out)
@@ -662,6 +714,129 @@ class HipOps:
             self._stream()), "fw_gemm_fp8")
         self._time_end(tok)
         return out
+
+    # ---- MXFP4 linear (include/fw_mi355x.h; no reference semantics) ------------------------------------------------------------------
+    def _mxfp4_empty(self, M, K):
+        """Unwritten MXFP4 rows on this device: (codes [M, Kp / 2], scales)."""
+        slabs = (K + 255) // 256
+        return (torch.empty(M, slabs * 128, dtype=torch.uint8, device=self.device),
+                torch.empty((M + 31) // 32, slabs, 32, 8, dtype=torch.uint8, device=self.device))
+
+    def quantize_mxfp4_rows(self, x):
+        """x bf16 / fp32 [M, K] (rows may be strided, any K) -> MXFP4Rows."""
+        if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or x.shape[1] < 1:
+            raise ValueError(f"bf16 / fp32 rows expected, got {x.dtype} {tuple(x.shape)} with strides {x.stride()}")
+        self._check_dev(x)
+        M, K = x.shape
+        q, s = self._mxfp4_empty(M, K)
+        _check(self.lib.fw_mxfp4_quant_rows(x.data_ptr(), max(x.stride(0), K), _dt(x), q.data_ptr(), q.stride(0), s.data_ptr(), M, K, self._stream()),
+               "fw_mxfp4_quant_rows")
+        return MXFP4Rows(q, s, K)
+
+    def dequantize_mxfp4_rows(self, mx, dtype=torch.bfloat16):
+        """MXFP4Rows -> [M, K] in bf16 or fp32 (exact in both)."""
+        self._check_dev(mx.q, mx.s)
+        y = torch.empty(mx.M, mx.K, dtype=dtype, device=self.device)
+        _check(self.lib.fw_mxfp4_dequant_rows(mx.q.data_ptr(), mx.q.stride(0), mx.s.data_ptr(), y.data_ptr(), mx.K, _dt(y), mx.M, mx.K, self._stream()),
+               "fw_mxfp4_dequant_rows")
+        return y
+
+    def pack_linear_mxfp4(self, w, b):
+        """w [N, K] (any K) -> LinearMXFP4: the fp32 / bf16 weights quantised along K, the bias in fp32."""
+        w = w.detach().to(device=self.device)
+        mx = self.quantize_mxfp4_rows(w if w.dtype == torch.bfloat16 else w.to(torch.float32))
+        return LinearMXFP4(mx.q, mx.s, None if b is None else self.to_f32(b), mx.K)
+
+    def linear_from_mxfp4(self, q, s, b, K):
+        """A linear whose weights are MXFP4 rows already (q, s as in MXFP4Rows; b fp32 [N] or None), without a copy."""
+        self._check_dev(q, s, b)
+        return LinearMXFP4(q, s, b, K)
+
+    def _linear_mxfp4(self, x, lin, act=None, g1=None, g0=None, res=None, out_f32=False, out=None, out_mxfp4=False):
+        """bf16 rows (quantised here) or MXFP4Rows x -> epilogue(x W^T): bf16, fp32 or MXFP4Rows."""
+        if not isinstance(x, MXFP4Rows):
+            if not torch.is_tensor(x) or x.dtype != torch.bfloat16:
+                raise ValueError(f"an MXFP4 linear takes bf16 rows or MXFP4Rows, got {getattr(x, 'dtype', type(x))}")
+            x = self.quantize_mxfp4_rows(x)
+        if x.K != lin.K:
+            raise ValueError(f"x has K = {x.K}, the linear K = {lin.K}")
+        self._check_dev(x.q, x.s, lin.q, lin.s, lin.b, g1, g0, res, out)
+        M, N = x.M, lin.N
+        for name, v in (("g1", g1), ("g0", g0)):
+            if v is not None and (v.dtype != torch.float32 or v.numel() != N or not v.is_contiguous()):
+                raise ValueError(f"{name}: contiguous fp32 [{N}] expected, got {v.dtype} {tuple(v.shape)}")
+        if res is not None and (res.shape != (M, N) or (N > 1 and res.stride(1) != 1)):
+            raise ValueError(f"res: [{M}, {N}] with contiguous rows expected, got {tuple(res.shape)} with strides {res.stride()}")
+        cs = None
+        if out_mxfp4:
+            if out is not None or out_f32:
+                raise ValueError("out_mxfp4 allocates its own output and excludes out_f32")
+            c, cs = self._mxfp4_empty(M, N)
+            ldc, odt = c.stride(0), FW_DT_MXFP4
+        else:
+            c = out if out is not None else torch.empty(M, N, dtype=torch.float32 if out_f32 else torch.bfloat16, device=self.device)
+            if c.shape != (M, N) or (N > 1 and c.stride(1) != 1):
+                raise ValueError(f"out: [{M}, {N}] with contiguous rows expected, got {tuple(c.shape)} with strides {c.stride()}")
+            ldc, odt = max(c.stride(0), N), _dt(c)
+        tok = None if self._timing is None else self._time_begin(
+            dict(kind="linear", M=M, N=N, K=x.K, res=res is not None, out_f32=odt == FW_DT_F32, act=act, mxfp4=True))
+        _check(self.lib.fw_gemm_mxfp4(
+            x.q.data_ptr(), x.q.stride(0), x.s.data_ptr(), lin.q.data_ptr(), lin.q.stride(0), lin.s.data_ptr(), c.data_ptr(), ldc, odt, _ptr(cs),
+            M, N, x.K, _ptr(lin.b), ACT[act], _ptr(g1), _ptr(g0), _ptr(res), 0 if res is None else max(res.stride(0), N),
+            FW_DT_NONE if res is None else _dt(res), self._stream()), "fw_gemm_mxfp4")
+        self._time_end(tok)
+        return MXFP4Rows(c, cs, N) if out_mxfp4 else c
+
+    def linear_mxfp4(self, x, lin, **kw):
+        """linear() for callers that want a refusal when `lin` is not an MXFP4 linear."""
+        if not lin.mxfp4:
+            raise ValueError("not an MXFP4 linear")
+        return self._linear_mxfp4(x, lin, **kw)
+
+    # ---- the seam between two halves of a block --------------------------------------------------------------------------------------
+    def residual_norm(self, x, y=None, bias=None, g1=None, g0=None, post=None, post_w=None, w=None, b=None, scale=None, shift=None,
+                      norm="layer", eps=1e-6, x_out=None, out="bf16"):
+        """x' = x + [post norm](y + bias) * g1 + g0, written to x_out (default: x, in place); -> h = norm(x') * w + b, * (1 + scale) + shift, as
+        bf16 rows or (out="mxfp4") MXFP4Rows.  y None: h alone.  x, x_out [rows, C] fp32 or bf16, y fp32 or bf16; bias / post_w / w / b [C];
+        g1 / g0 / scale / shift [C] or [groups, C] with rows % groups == 0: equal runs of rows share a vector.  post: None, "layer" or "rms"
+        (post_w only with it); norm: "layer" or "rms" (b only with w)."""
+        if x.dim() != 2 or x.dtype not in (torch.float32, torch.bfloat16) or (x.shape[1] > 1 and x.stride(1) != 1) or x.shape[1] < 1:
+            raise ValueError(f"x: fp32 / bf16 rows expected, got {x.dtype} {tuple(x.shape)} with strides {x.stride()}")
+        if out not in ("bf16", "mxfp4") or norm not in ("layer", "rms") or post not in RNORM:
+            raise ValueError(f"out: 'bf16' | 'mxfp4', norm: 'layer' | 'rms', post: None | 'layer' | 'rms'; got {out!r}, {norm!r}, {post!r}")
+        rows, C = x.shape
+        if y is None:
+            bias = g1 = g0 = post_w = x_out = None
+            post = None
+        else:
+            x_out = x if x_out is None else x_out
+            for name, v in (("y", y), ("x_out", x_out)):
+                if v.shape != x.shape or (C > 1 and v.stride(1) != 1) or (name == "x_out" and v.dtype != x.dtype):
+                    raise ValueError(f"{name}: rows of x's shape expected, got {v.dtype} {tuple(v.shape)} with strides {v.stride()}")
+        groups = 1
+        for name, v in (("g1", g1), ("g0", g0), ("scale", scale), ("shift", shift)):
+            if v is not None and v.dim() == 2 and v.shape[0] > 1:
+                if groups not in (1, v.shape[0]) or rows % v.shape[0]:
+                    raise ValueError(f"{name}: {v.shape[0]} vectors for {rows} rows in {groups} group(s)")
+                groups = v.shape[0]
+        for name, v, n in (("bias", bias, 1), ("post_w", post_w, 1), ("w", w, 1), ("b", b, 1), ("g1", g1, groups), ("g0", g0, groups),
+                           ("scale", scale, groups), ("shift", shift, groups)):
+            if v is not None and (v.dtype != torch.float32 or not v.is_contiguous() or v.numel() != n * C or v.shape[-1] != C):
+                raise ValueError(f"{name}: contiguous fp32 [{C}]" + (f" or [{n}, {C}]" if n > 1 else "") + f" expected, got {v.dtype} {tuple(v.shape)}")
+        if post in (None, "none"):
+            post_w = None
+        self._check_dev(x, y, bias, g1, g0, post_w, w, b, scale, shift, x_out)
+        hs = None
+        if out == "mxfp4":
+            h, hs = self._mxfp4_empty(rows, C)
+        else:
+            h = torch.empty(rows, C, dtype=torch.bfloat16, device=self.device)
+        _check(self.lib.fw_residual_norm(
+            x.data_ptr(), max(x.stride(0), C), _ptr(x_out), 0 if x_out is None else max(x_out.stride(0), C), _dt(x),
+            _ptr(y), 0 if y is None else max(y.stride(0), C), FW_DT_NONE if y is None else _dt(y), _ptr(bias), _ptr(g1), _ptr(g0), RNORM[post], _ptr(post_w),
+            RNORM[norm], _ptr(w), _ptr(b), _ptr(scale), _ptr(shift), float(eps), h.data_ptr(), h.stride(0), FW_DT_MXFP4 if hs is not None else FW_DT_BF16,
+            _ptr(hs), rows, C, max(1, rows // groups), self._stream()), "fw_residual_norm")
+        return MXFP4Rows(h, hs, C) if hs is not None else h
 
     # ---- fp8 attention (hd 128; parity unpinned: no reference semantics, see include/fw_mi355x.h) ---------------------------
     FP8_Q_EXP = 3      # Q8 holds q * softmax_scale * log2(e) * 2^3

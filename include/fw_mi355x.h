@@ -35,6 +35,7 @@ extern "C" {
 #define FW_DT_NONE 0
 #define FW_DT_BF16 1
 #define FW_DT_F32  2
+#define FW_DT_MXFP4 3  /* an OUTPUT held as MXFP4 rows: fw_gemm_mxfp4, fw_residual_norm */
 
 /* activation applied to (acc + bias) in fw_gemm_bf16 / fw_gemv_f32 */
 #define FW_ACT_NONE      0
@@ -451,6 +452,51 @@ int fw_gemm_fp8(const uint8_t* A, int64_t lda, const uint8_t* W, int64_t ldw, co
                 void* C, int64_t ldc, int out_dtype, int M, int N, int K,
                 const float* bias, int act, const float* g1, const float* g0,
                 const void* res, int64_t ldr, int res_dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * MXFP4 linear: weights AND activations as OCP microscaled 4-bit floating point (Microscaling Formats v1.0) -- 32 consecutive e2m1 values
+ * along K share one E8M0 scale, a power of two.  The reference has no 4-bit path: these semantics are this library's own.
+ *   scale of a block: 2^(E - 2), E the exponent of its largest magnitude; 2^(E - 1) where that magnitude's mantissa is 1.75 or above (it
+ *     would round past 6, the largest e2m1 value); within 2^-127 .. 2^125.  A block that holds an infinity or NaN gets the NaN scale 0xff:
+ *     it decodes to NaN and every product with it is NaN.
+ *   value: e2m1(v / scale), to nearest, ties to the even code; values above 6 scales saturate.
+ * Storage ("MXFP4 rows", M x K): codes q [M][ldq] bytes, two values a byte with the first in the low half, K padded with zeros to
+ *   Kp = roundup(K, 256): ldq >= Kp / 2, ldq % 16 == 0, q 16-byte aligned; scales s [ceil(M / 32)][Kp / 256][32][8] bytes, contiguous, 4-byte
+ *   aligned: s[r / 32][k / 256][r % 32][k / 32 % 8].  Scale bytes of rows past M inside the last group of 32 are not read as values.
+ * ------------------------------------------------------------------------------------------------------------- */
+
+/* x [M][K] (bf16 or f32, ldx elements, any K and alignment of the element type) -> MXFP4 rows.  8 values per access where K % 8 == 0 and
+ * the rows are 16-byte aligned, one at a time otherwise. */
+int fw_mxfp4_quant_rows(const void* x, int64_t ldx, int x_dtype, uint8_t* q, int64_t ldq, uint8_t* s, int M, int K, void* stream);
+
+/* MXFP4 rows -> y [M][K] (bf16 or f32; exact in both). */
+int fw_mxfp4_dequant_rows(const uint8_t* q, int64_t ldq, const uint8_t* s, void* y, int64_t ldy, int y_dtype, int M, int K, void* stream);
+
+/* C[M][N] = epi(A[M][K] W[N][K]^T + bias): both operands MXFP4 rows, block scales applied by the MFMA, fp32 accumulation, then
+ * fw_gemm_bf16's epilogue (bias -> act -> per-column affine g1 / g0 -> + residual -> out_dtype).  C may alias res.
+ * out_dtype FW_DT_MXFP4: the result is rounded to bf16 and quantised along N by the rule above -- the bytes of fw_mxfp4_quant_rows on the
+ * bf16 output -- C = codes [M][ldc] (bytes), cs = scales; the input of the next MXFP4 linear without a pass of its own (cs is not used
+ * for the other types).  lda, ldw (bytes) < 2^23. */
+int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, const uint8_t* W, int64_t ldw, const uint8_t* sw,
+                  void* C, int64_t ldc, int out_dtype, uint8_t* cs, int M, int N, int K,
+                  const float* bias, int act, const float* g1, const float* g0,
+                  const void* res, int64_t ldr, int res_dtype, void* stream);
+
+/* The seam between two halves of a block in one pass: the gated residual update that ends one half and the norm that opens the next.
+ *   t  = y + bias;  post: t = norm_post(t) * post_w;  x' = x + t * g1 + g0  (written to x_out, which may be x);
+ *   h  = norm(x') [* w [+ b]];  h = h * (1 + scale) + shift                  (bf16, or MXFP4 rows of the bf16 value)
+ * norm / post: LAYER = (v - mean) / sqrt(var + eps), RMS = v / sqrt(mean square + eps); post also NONE.  The norm reads x' as it is stored.
+ * x / x_out [rows][C] f32 or bf16 (one type), y f32 or bf16; y NULL: no update, h = norm(x) alone (bias, g1, g0, post, x_out unused).
+ * g1, g0, scale, shift: [ceil(rows / rows_per_mod)][C] fp32, row r uses vector r / rows_per_mod (one vector for all: rows_per_mod >= rows);
+ * bias, post_w, w, b: [C] fp32; NULL = absent.  C <= 8192.
+ * With C = 1024 or 5120, fp32 x, LAYER and no post norm: the bits of fw_residual_add followed by fw_layernorm_mod. */
+#define FW_RNORM_NONE  0
+#define FW_RNORM_LAYER 1
+#define FW_RNORM_RMS   2
+int fw_residual_norm(const void* x, int64_t ldx, void* x_out, int64_t ldxo, int x_dtype, const void* y, int64_t ldy, int y_dtype,
+                     const float* bias, const float* g1, const float* g0, int post, const float* post_w,
+                     int norm, const float* w, const float* b, const float* scale, const float* shift, float eps,
+                     void* h, int64_t ldh, int h_dtype, uint8_t* h_scale, int rows, int C, int rows_per_mod, void* stream);
 
 #ifdef __cplusplus
 }
