@@ -48,103 +48,135 @@ __device__ __forceinline__ void mx_tile(const MxArgs& p, int& tm, int& tn) {
     tn = in_g / gsz;
 }
 
-// One 64 x 64 quadrant of a wave: accumulators [2][2] -> LDS (16 KiB of this wave's own) -> rows -> bias, activation, per-column affine,
-// residual, store.  A lane owns 8 consecutive columns of one row at a time, 8 rows per step: 16-byte stores in bf16, and with MXFP4 output
-// a block of 32 columns is the 4 lanes of a quad.
-template <int ACT>
-__device__ __forceinline__ void mx_epilogue64(const MxArgs& p, char* reg, const f32x16_t& a00, const f32x16_t& a01, const f32x16_t& a10,
-                                              const f32x16_t& a11, int lane, int m0, int n0) {
-    const int fi = lane & 31, hi = lane >> 5;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int row_l = (r & 3) + 8 * (r >> 2) + 4 * hi;
-        *(float*)(reg + row_l * 256 + fi * 4) = a00[r];
-        *(float*)(reg + row_l * 256 + (32 + fi) * 4) = a01[r];
-        *(float*)(reg + (32 + row_l) * 256 + fi * 4) = a10[r];
-        *(float*)(reg + (32 + row_l) * 256 + (32 + fi) * 4) = a11[r];
-    }
-    const int c8 = (lane & 7) * 8, rl = lane >> 3;
-    const int col = n0 + c8;
+// Epilogue of NQ quadrants (64 x 64 each, stacked along M) of a wave: accumulators -> LDS (16 KiB of the wave's own) -> rows -> bias,
+// activation, per-column affine, residual, store.  A lane owns 8 consecutive columns of a row, 8 rows per step: 16-byte accesses in bf16,
+// and with MXFP4 output a block of 32 columns is the 4 lanes of a quad.
+// LDS image: 16-byte chunk c of row r lies at (c >> 1) + 8 ((c ^ r) & 1) of the row's 16: the 16 lanes of a read (chunk 2q or 2q + 1 of two
+// neighbouring rows) then hit 16 different chunks of the 64 banks.
+// ACT, RES < 0: decided per element at run time.  VEC: every row of C and of the residual is 16-byte accessible and N % 8 == 0.
+// With a residual the 64 rows' loads are all in flight before the transpose, and the next quadrant's are issued as registers free up:
+// read one step at a time they cost a memory latency each (32 us per 256 x 256 tile with an fp32 residual, against 32 us of main loop).
+template <int ACT, int RES, bool VEC, int NQ, typename Acc>
+__device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Acc& acc, int lane, int m0, int n0) {
+    const int fi = lane & 31, hi = lane >> 5, q = lane & 7, rl = lane >> 3;
+    const int col = n0 + q * 8;
+    const bool in = col < p.N;
+    const int res_dtype = RES < 0 ? p.res_dtype : RES;
     float bias[8], g1[8], g0[8];
+    const bool affine = p.g1 || p.g0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const bool in = col + j < p.N;
-        bias[j] = p.bias && in ? p.bias[col + j] : 0.f;
-        g1[j] = p.g1 && in ? p.g1[col + j] : 1.f;
-        g0[j] = p.g0 && in ? p.g0[col + j] : 0.f;
+        bias[j] = p.bias && col + j < p.N ? p.bias[col + j] : 0.f;
+        g1[j] = p.g1 && col + j < p.N ? p.g1[col + j] : 1.f;
+        g0[j] = p.g0 && col + j < p.N ? p.g0[col + j] : 0.f;
     }
-#pragma unroll 2
-    for (int it = 0; it < 8; ++it) {
-        const int row_l = it * 8 + rl, row = m0 + row_l;
-        const f32x4_t lo = *(const f32x4_t*)(reg + row_l * 256 + c8 * 4), up = *(const f32x4_t*)(reg + row_l * 256 + c8 * 4 + 16);
-        float v[8] = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = fw_apply_act(v[j] + bias[j], ACT);
-            if (p.g1 || p.g0) v[j] = fw_affine(v[j], g1[j], g0[j]);
+    u32x4_t rv[8][RES == FW_DT_F32 ? 2 : 1];
+    auto load_res = [&](int it, int row) __attribute__((always_inline)) {
+        if (VEC && RES > 0 && in && row < p.M) {
+            const char* r = (const char*)p.res + ((int64_t)row * p.ldr + col) * (RES == FW_DT_F32 ? 4 : 2);
+            rv[it][0] = *(const u32x4_t*)r;
+            if (RES == FW_DT_F32) rv[it][RES == FW_DT_F32 ? 1 : 0] = *(const u32x4_t*)(r + 16);
         }
-        const bool live = row < p.M;
-        if (p.res_dtype != FW_DT_NONE && live) {
-            const int64_t o = (int64_t)row * p.ldr + col;
-            if (p.vec && col < p.N) {
-                if (p.res_dtype == FW_DT_F32) {
-                    const f32x4_t x = *(const f32x4_t*)((const float*)p.res + o), y = *(const f32x4_t*)((const float*)p.res + o + 4);
+    };
+    if (VEC && RES > 0) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) { v[j] += x[j]; v[4 + j] += y[j]; }
-                } else {
-                    const u32x4_t w = *(const u32x4_t*)((const uint16_t*)p.res + o);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) { v[2 * j] += __uint_as_float(w[j] << 16); v[2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u); }
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (col + j < p.N) v[j] += p.res_dtype == FW_DT_F32 ? ((const float*)p.res)[o + j] : bf16_bits_to_f32(((const uint16_t*)p.res)[o + j]);
-            }
-        }
-        if (p.out_dtype == FW_DT_MXFP4) {
-            // the value is rounded to bf16 first: a fused quantisation returns the bytes of fw_mxfp4_quant_rows on the bf16 output.
-            // Columns past N are zeros of the padded row (the launcher's grid covers all of it).
-            u32x4_t h;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) h[j] = pack_bf16x2(col + 2 * j < p.N ? v[2 * j] : 0.f, col + 2 * j + 1 < p.N ? v[2 * j + 1] : 0.f);
-            const uint32_t byte = mx_scale_byte(mx_quad_max(mx_top8_bf16(h)));
-            const uint32_t codes = mx_pack8_bf16(h, mx_scale_f32(byte));
-            if (live && col < p.cslabs * MX_SLAB) {
-                *(uint32_t*)((uint8_t*)p.C + (int64_t)row * p.ldc + (col >> 1)) = codes;
-                if ((lane & 3) == 0) p.cs[((int64_t)(row >> 5) * p.cslabs + (col >> 8)) * 256 + (row & 31) * 8 + ((col >> 5) & 7)] = (uint8_t)byte;
-            }
-        } else if (live) {
-            const int64_t o = (int64_t)row * p.ldc + col;
-            if (p.out_dtype == FW_DT_F32) {
-                if (p.vec && col < p.N) {
-                    *(f32x4_t*)((float*)p.C + o) = f32x4_t{v[0], v[1], v[2], v[3]};
-                    *(f32x4_t*)((float*)p.C + o + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) if (col + j < p.N) ((float*)p.C)[o + j] = v[j];
-                }
-            } else {
-                if (p.vec && col < p.N) {
-                    *(u32x4_t*)((uint16_t*)p.C + o) = u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) if (col + j < p.N) ((uint16_t*)p.C)[o + j] = f32_to_bf16_bits(v[j]);
-                }
-            }
-        }
+        for (int it = 0; it < 8; ++it) load_res(it, m0 + it * 8 + rl);
     }
+    auto quadrant = [&](auto q_tag) __attribute__((always_inline)) {
+        constexpr int Q = decltype(q_tag)::value;
+        // chunk of column fi: fi >> 2, of column 32 + fi: 8 + (fi >> 2); rows of a register pair alternate in parity
+        const int c = fi >> 2, base = (4 * hi) * 256 + (fi & 3) * 4 + (c >> 1) * 16;
+        const int at[2] = {base + (c & 1) * 128, base + ((c & 1) ^ 1) * 128};
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row_l = rb * 32 + (r & 3) + 8 * (r >> 2);
+                *(float*)(reg + row_l * 256 + at[r & 1]) = acc[2 * Q + rb][0][r];
+                *(float*)(reg + row_l * 256 + at[r & 1] + 64) = acc[2 * Q + rb][1][r];
+            }
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+            const int row_l = it * 8 + rl, row = m0 + Q * 64 + row_l;
+            const f32x4_t lo = *(const f32x4_t*)(reg + row_l * 256 + q * 16 + (rl & 1) * 128), up = *(const f32x4_t*)(reg + row_l * 256 + q * 16 + ((rl & 1) ^ 1) * 128);
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = fw_apply_act(v[j] + bias[j], ACT < 0 ? p.act : ACT);
+            if (affine) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = fw_affine(v[j], g1[j], g0[j]);
+            }
+            const bool live = row < p.M;
+            if (VEC && RES > 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (RES == FW_DT_F32) { v[j] += __uint_as_float(rv[it][0][j]); v[4 + j] += __uint_as_float(rv[it][RES == FW_DT_F32 ? 1 : 0][j]); }
+                    else { v[2 * j] += __uint_as_float(rv[it][0][j] << 16); v[2 * j + 1] += __uint_as_float(rv[it][0][j] & 0xffff0000u); }
+                }
+                if (Q + 1 < NQ) load_res(it, row + 64);
+            } else if (res_dtype != FW_DT_NONE && live) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t o = (int64_t)row * p.ldr + col + j;
+                    if (col + j < p.N) v[j] += res_dtype == FW_DT_F32 ? ((const float*)p.res)[o] : bf16_bits_to_f32(((const uint16_t*)p.res)[o]);
+                }
+            }
+            if (p.out_dtype == FW_DT_MXFP4) {
+                // the value is rounded to bf16 first: a fused quantisation returns the bytes of fw_mxfp4_quant_rows on the bf16 output.
+                // Columns past N are zeros of the padded row (the launcher's grid covers all of it).
+                u32x4_t h;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    h[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+                    if (VEC) { if (!in) h[j] = 0; }
+                    else h[j] &= (col + 2 * j < p.N ? 0xffffu : 0u) | (col + 2 * j + 1 < p.N ? 0xffff0000u : 0u);
+                }
+                const uint32_t byte = mx_scale_byte(mx_quad_max(mx_top8_bf16(h)));
+                const uint32_t codes = mx_pack8_bf16(h, mx_scale_f32(byte));
+                if (live && col < p.cslabs * MX_SLAB) {
+                    *(uint32_t*)((uint8_t*)p.C + (int64_t)row * p.ldc + (col >> 1)) = codes;
+                    if ((lane & 3) == 0) p.cs[((int64_t)(row >> 5) * p.cslabs + (col >> 8)) * 256 + (row & 31) * 8 + ((col >> 5) & 7)] = (uint8_t)byte;
+                }
+            } else if (live && in) {
+                const int64_t o = (int64_t)row * p.ldc + col;
+                if (VEC) {
+                    if (p.out_dtype == FW_DT_F32) {
+                        *(f32x4_t*)((float*)p.C + o) = f32x4_t{v[0], v[1], v[2], v[3]};
+                        *(f32x4_t*)((float*)p.C + o + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+                    } else {
+                        *(u32x4_t*)((uint16_t*)p.C + o) = u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (col + j < p.N) {
+                            if (p.out_dtype == FW_DT_F32) ((float*)p.C)[o + j] = v[j];
+                            else ((uint16_t*)p.C)[o + j] = f32_to_bf16_bits(v[j]);
+                        }
+                }
+            }
+        }
+    };
+    quadrant(std::integral_constant<int, 0>{});
+    if constexpr (NQ > 1) quadrant(std::integral_constant<int, 1>{});
 }
 
-template <typename F>
-__device__ __forceinline__ void mx_by_act(int act, F&& f) {
-    switch (act) {
-        case FW_ACT_RELU: f(std::integral_constant<int, FW_ACT_RELU>{}); break;
-        case FW_ACT_GELU_TANH: f(std::integral_constant<int, FW_ACT_GELU_TANH>{}); break;
-        case FW_ACT_GELU_ERF: f(std::integral_constant<int, FW_ACT_GELU_ERF>{}); break;
-        case FW_ACT_SILU: f(std::integral_constant<int, FW_ACT_SILU>{}); break;
-        default: f(std::integral_constant<int, FW_ACT_NONE>{}); break;
-    }
+// The combinations the engine runs are compiled on their own (each activation without a residual, either residual without an activation);
+// the others, and rows that cannot be accessed 16 bytes at a time, decide per element.
+template <int NQ, typename Acc>
+__device__ __forceinline__ void mx_finish(const MxArgs& p, char* reg, const Acc& acc, int lane, int m0, int n0) {
+    if (!p.vec) { mx_epilogue<-1, -1, false, NQ>(p, reg, acc, lane, m0, n0); return; }
+    if (p.res_dtype == FW_DT_NONE) {
+        switch (p.act) {
+            case FW_ACT_RELU: mx_epilogue<FW_ACT_RELU, 0, true, NQ>(p, reg, acc, lane, m0, n0); break;
+            case FW_ACT_GELU_TANH: mx_epilogue<FW_ACT_GELU_TANH, 0, true, NQ>(p, reg, acc, lane, m0, n0); break;
+            case FW_ACT_GELU_ERF: mx_epilogue<FW_ACT_GELU_ERF, 0, true, NQ>(p, reg, acc, lane, m0, n0); break;
+            case FW_ACT_SILU: mx_epilogue<FW_ACT_SILU, 0, true, NQ>(p, reg, acc, lane, m0, n0); break;
+            default: mx_epilogue<FW_ACT_NONE, 0, true, NQ>(p, reg, acc, lane, m0, n0); break;
+        }
+    } else if (p.act != FW_ACT_NONE) mx_epilogue<-1, -1, true, NQ>(p, reg, acc, lane, m0, n0);
+    else if (p.res_dtype == FW_DT_F32) mx_epilogue<FW_ACT_NONE, FW_DT_F32, true, NQ>(p, reg, acc, lane, m0, n0);
+    else mx_epilogue<FW_ACT_NONE, FW_DT_BF16, true, NQ>(p, reg, acc, lane, m0, n0);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -216,9 +248,166 @@ __global__ __launch_bounds__(256, 2) void gemm_mxfp4_128_kernel(MxArgs p) {
 #undef FWX_STEP
     }
     __syncthreads();                                      // everybody has read the last slab: the stages become the epilogue's space
-    mx_by_act(p.act, [&](auto act) __attribute__((always_inline)) {
-        mx_epilogue64<decltype(act)::value>(p, smem + wave * 16384, acc[0][0], acc[0][1], acc[1][0], acc[1][1], lane, m0 + wm * 64, n0 + wn * 64);
-    });
+    mx_finish<1>(p, smem + wave * 16384, acc, lane, m0 + wm * 64, n0 + wn * 64);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// 256 x 256 tile, 8 waves = 2 (M) x 4 (N) with wave tiles of 128 x 64, the two 4-wave groups one barrier slot apart:
+//     slot:        2t          2t+1         2t+2         2t+3
+//     group A:   LOAD(t)     MFMA(t)      LOAD(t+1)    MFMA(t+1)          LOAD(t): W fragments and A rows 0..63 of the wave tile, then this
+//     group B:   MFMA(t-1)   LOAD(t)      MFMA(t)      LOAD(t+1)          wave's scale dwords and 8 DMA pieces; MFMA(t): 32 MFMAs in one
+//                                                                         burst, A rows 64..127 re-read into the registers it has consumed
+// so a SIMD always has one wave in its burst while the other one reads.  A in two 32 KiB stages, W in three (160 KiB): with the third, W(t+2)
+// can be requested while W(t+1) waits.  Scale dwords go from memory to registers one slab ahead; they are requested ahead of the slab's
+// pieces, so the counted wait for the pieces covers them.  Waits: a wave's requests in LOAD(t) are S(t+1) 6, A(t+1) 4, W(t+2) 4;
+// vmcnt(4) at the end of the burst = everything but W(t+2) has landed; group B's W(t+1) is read one slot after its LOAD(t) by group A, so it
+// waits vmcnt(14) there = all but this LOAD's own.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int LM = 256, LN = 256;
+constexpr int L_A_STAGE = LM * 128, L_W_BASE = 2 * L_A_STAGE, L_W_STAGE = LN * 128, L_LDS = L_W_BASE + 3 * L_W_STAGE;
+
+#define FWX_BARRIER() do { __builtin_amdgcn_sched_barrier(0); asm volatile("s_barrier" ::: "memory"); __builtin_amdgcn_sched_barrier(0); } while (0)
+template <int N> __device__ __forceinline__ void mx_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+__global__ __launch_bounds__(512, 2) void gemm_mxfp4_256_kernel(MxArgs p) {
+    __shared__ __attribute__((aligned(16))) char smem[L_LDS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int grp = wave >> 2, wn = wave & 3, fi = lane & 31, hi = lane >> 5;
+    int tm, tn;
+    mx_tile(p, tm, tn);
+    const int m0 = tm * LM, n0 = tn * LN;
+    const auto ars = mx_rsrc(p.A + (int64_t)m0 * p.lda, (long long)(p.M - m0) * p.lda);
+    const auto wrs = mx_rsrc(p.W + (int64_t)n0 * p.ldw, (long long)(p.N - n0) * p.ldw);
+    // scale tiles of this wave's 4 + 2 groups of 32 rows; groups past the end read zeros
+    const int sstride = __builtin_amdgcn_readfirstlane(p.slabs * 256);
+    const int ab = (m0 >> 5) + grp * 4, wb = (n0 >> 5) + wn * 2;
+    const auto sars = mx_rsrc(p.sa + (int64_t)ab * sstride, (long long)((p.M + 31) / 32 - ab) * sstride);
+    const auto swrs = mx_rsrc(p.sw + (int64_t)wb * sstride, (long long)((p.N + 31) / 32 - wb) * sstride);
+    const int svo = fi * 8 + hi * 4;
+    // a piece = 8 rows x 128 bytes; this wave's pieces: tile rows (grp * 128 + 32 wn) .. + 31 of both operands
+    const int pr = lane >> 3, pc = lane & 7;
+    const int va[2] = {pr * (int)p.lda + ((pc ^ (pr >> 1)) << 4), pr * (int)p.lda + ((pc ^ ((pr >> 1) | 4)) << 4)};
+    const int vw[2] = {pr * (int)p.ldw + ((pc ^ (pr >> 1)) << 4), pr * (int)p.ldw + ((pc ^ ((pr >> 1) | 4)) << 4)};
+    const int astep = __builtin_amdgcn_readfirstlane((int)p.lda * 8), wstep = __builtin_amdgcn_readfirstlane((int)p.ldw * 8);
+    const int q0 = grp * 16 + 4 * wn;
+    auto issue_a = [&](int as, int kt) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) FWX_BLDS16(ars, va[j & 1], kt * 128 + (q0 + j) * astep, smem + as * L_A_STAGE + (q0 + j) * 1024);
+    };
+    auto issue_w = [&](int ws, int kt) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) FWX_BLDS16(wrs, vw[j & 1], kt * 128 + (q0 + j) * wstep, smem + L_W_BASE + ws * L_W_STAGE + (q0 + j) * 1024);
+    };
+    auto load_scales = [&](int (&sa)[4], int (&sw)[2], int kt) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sa[i] = (int)__builtin_amdgcn_raw_buffer_load_b32(sars, svo, i * sstride + kt * 256, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) sw[i] = (int)__builtin_amdgcn_raw_buffer_load_b32(swrs, svo, i * sstride + kt * 256, 0);
+    };
+    const int swz = (fi >> 1) & 7;
+    int co[4];                             // byte offset of k-step j's chunk inside a row
+#pragma unroll
+    for (int j = 0; j < 4; ++j) co[j] = ((4 * hi + j) ^ swz) << 4;
+    const int a_row = (grp * 128 + fi) * 128, w_row = L_W_BASE + (wn * 64 + fi) * 128;
+
+    f32x16_t acc[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    i32x4_t af[2][4], wf[2][4];            // [row / column block][k-step]
+    int sa[4], sw[2], na[4], nw[2];        // scales of this slab and of the next
+
+    const int nk = p.slabs;                // >= 4 (launcher)
+    load_scales(sa, sw, 0);
+    load_scales(na, nw, 1);
+    issue_a(0, 0); issue_w(0, 0);
+    issue_a(1, 1); issue_w(1, 1);
+    issue_w(2, 2);
+    mx_wait_vm<12>();
+    FWX_BARRIER();
+    if (grp == 1) FWX_BARRIER();
+
+    int kt = 0, ws = 0;                    // ws = kt % 3
+    // One slab.  The peeling is compile-time (first / steady / second-last / last), so LOAD and MFMA are one basic block each; the
+    // accumulators are pinned by empty asm, which keeps the burst on its side of the barrier behind it.
+    auto slab = [&](auto g_tag, auto first_tag, auto n1_tag, auto n2_tag) __attribute__((always_inline)) {
+        constexpr int G = decltype(g_tag)::value;
+        constexpr bool FIRST = decltype(first_tag)::value, N1 = decltype(n1_tag)::value, N2 = decltype(n2_tag)::value;   // kt == 0; kt + 1 < nk; kt + 2 < nk
+        const int as = kt & 1;
+        const char* ab_ = smem + as * L_A_STAGE + a_row;
+        const char* wb_ = smem + ws * L_W_STAGE + w_row;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            wf[0][j] = *(const i32x4_t*)(wb_ + co[j]);
+            wf[1][j] = *(const i32x4_t*)(wb_ + 32 * 128 + co[j]);
+            af[0][j] = *(const i32x4_t*)(ab_ + co[j]);
+            af[1][j] = *(const i32x4_t*)(ab_ + 32 * 128 + co[j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (!FIRST && N1) {
+            load_scales(na, nw, kt + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            issue_a(as ^ 1, kt + 1);
+            if (N2) issue_w(ws == 0 ? 2 : ws - 1, kt + 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (G == 1 && N1) {
+            if (FIRST) mx_wait_vm<4>(); else if (N2) mx_wait_vm<14>(); else mx_wait_vm<10>();
+        }
+        FWX_BARRIER();
+        __builtin_amdgcn_s_setprio(1);
+#define FWX_LOWER(J) do { \
+            acc[0][0] = FWX_MFMA(af[0][J], wf[0][J], acc[0][0], J, sa[0], sw[0]); \
+            acc[0][1] = FWX_MFMA(af[0][J], wf[1][J], acc[0][1], J, sa[0], sw[1]); \
+            __builtin_amdgcn_sched_barrier(0); \
+            af[0][J] = *(const i32x4_t*)(ab_ + 64 * 128 + co[J]); \
+            __builtin_amdgcn_sched_barrier(0); \
+            acc[1][0] = FWX_MFMA(af[1][J], wf[0][J], acc[1][0], J, sa[1], sw[0]); \
+            acc[1][1] = FWX_MFMA(af[1][J], wf[1][J], acc[1][1], J, sa[1], sw[1]); \
+            __builtin_amdgcn_sched_barrier(0); \
+            af[1][J] = *(const i32x4_t*)(ab_ + 96 * 128 + co[J]); \
+            __builtin_amdgcn_sched_barrier(0); } while (0)
+#define FWX_UPPER(J) do { \
+            acc[2][0] = FWX_MFMA(af[0][J], wf[0][J], acc[2][0], J, sa[2], sw[0]); \
+            acc[2][1] = FWX_MFMA(af[0][J], wf[1][J], acc[2][1], J, sa[2], sw[1]); \
+            acc[3][0] = FWX_MFMA(af[1][J], wf[0][J], acc[3][0], J, sa[3], sw[0]); \
+            acc[3][1] = FWX_MFMA(af[1][J], wf[1][J], acc[3][1], J, sa[3], sw[1]); } while (0)
+        FWX_LOWER(0); FWX_LOWER(1); FWX_LOWER(2); FWX_LOWER(3);
+        FWX_UPPER(0); FWX_UPPER(1); FWX_UPPER(2); FWX_UPPER(3);
+#undef FWX_LOWER
+#undef FWX_UPPER
+        __builtin_amdgcn_s_setprio(0);
+        asm volatile("" : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1]));
+        asm volatile("" : "+v"(acc[2][0]), "+v"(acc[2][1]), "+v"(acc[3][0]), "+v"(acc[3][1]));
+        if (N1) {
+            if (N2) mx_wait_vm<4>(); else mx_wait_vm<0>();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sa[i] = na[i];
+            sw[0] = nw[0]; sw[1] = nw[1];
+        }
+        FWX_BARRIER();
+        ++kt;
+        ws = ws == 2 ? 0 : ws + 1;
+    };
+    using T = std::true_type;
+    using F = std::false_type;
+    auto mainloop = [&](auto g_tag) __attribute__((always_inline)) {
+        // (distinct opaque markers at both ends of an arm keep the compiler from hoisting the arms' common head above the group branch
+        //  and from merging their tails)
+        asm volatile("; mxfp4 two-slot mainloop, group %0: begin" ::"n"(decltype(g_tag)::value) : "memory");
+        slab(g_tag, T{}, T{}, T{});
+        while (kt < nk - 2) slab(g_tag, F{}, T{}, T{});
+        slab(g_tag, F{}, T{}, F{});                           // kt = nk - 2
+        slab(g_tag, F{}, F{}, F{});                           // kt = nk - 1
+        asm volatile("; mxfp4 two-slot mainloop, group %0: end" ::"n"(decltype(g_tag)::value) : "memory");
+    };
+    if (grp == 0) { mainloop(std::integral_constant<int, 0>{}); FWX_BARRIER(); }
+    else mainloop(std::integral_constant<int, 1>{});
+    mx_finish<2>(p, smem + wave * 16384, acc, lane, m0 + grp * 128, n0 + wn * 64);
 }
 
 }  // namespace
@@ -251,9 +440,31 @@ extern "C" int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, c
     p.vec = (N % 8) == 0 && (out_dtype == FW_DT_MXFP4 || ((ldc % ce) == 0 && (((uintptr_t)C) & 15) == 0)) &&
             (res_dtype == FW_DT_NONE || ((ldr % re) == 0 && (((uintptr_t)res) & 15) == 0));
     const int n_cover = out_dtype == FW_DT_MXFP4 ? cslabs * MX_SLAB : N;       // the padding of a quantised row is written too
-    p.tiles_m = (M + SM - 1) / SM; p.tiles_n = (n_cover + SN - 1) / SN;
+    hipStream_t st = (hipStream_t)stream;
+    // 256 x 256 tiles from two full rounds' worth of rows and columns on; below, and for a tail of at most 128 rows past the last full
+    // tile (a whole extra round of 256-row tiles otherwise), the 128 x 128 kernel.  Both add the same instructions in the same order per
+    // output element: a row's bits do not depend on the kernel that computes it.
+    int m_big = 0;
+    if (M >= 2048 && N >= 1024 && slabs >= 4) {
+        const int tail = M % LM;
+        m_big = tail > 0 && tail <= SM ? M - tail : M;
+        MxArgs b = p;
+        b.M = m_big;
+        b.tiles_m = (m_big + LM - 1) / LM; b.tiles_n = (n_cover + LN - 1) / LN;
+        const int64_t nwg = (int64_t)b.tiles_m * b.tiles_n;
+        if (nwg > 0x7fffffff) { fw_set_error("fw_gemm_mxfp4: grid too large"); return FW_E_BADARG; }
+        hipLaunchKernelGGL(gemm_mxfp4_256_kernel, dim3((unsigned)nwg), dim3(512), 0, st, b);
+        const int rc = (int)hipGetLastError();
+        if (rc || m_big == M) return rc;
+    }
+    // the rest: a multiple of 32 rows in, so scale tiles and quantised output start on a tile of their own
+    p.A = A + (int64_t)m_big * lda; p.sa = sa + (int64_t)(m_big / 32) * slabs * 256; p.M = M - m_big;
+    if (out_dtype == FW_DT_MXFP4) { p.C = (uint8_t*)C + (int64_t)m_big * ldc; p.cs = cs + (int64_t)(m_big / 32) * cslabs * 256; }
+    else p.C = (char*)C + (int64_t)m_big * ldc * (out_dtype == FW_DT_F32 ? 4 : 2);
+    if (res_dtype != FW_DT_NONE) p.res = (const char*)res + (int64_t)m_big * ldr * (res_dtype == FW_DT_F32 ? 4 : 2);
+    p.tiles_m = (p.M + SM - 1) / SM; p.tiles_n = (n_cover + SN - 1) / SN;
     const int64_t nwg = (int64_t)p.tiles_m * p.tiles_n;
     if (nwg > 0x7fffffff) { fw_set_error("fw_gemm_mxfp4: grid too large"); return FW_E_BADARG; }
-    hipLaunchKernelGGL(gemm_mxfp4_128_kernel, dim3((unsigned)nwg), dim3(256), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL(gemm_mxfp4_128_kernel, dim3((unsigned)nwg), dim3(256), 0, st, p);
     return (int)hipGetLastError();
 }
