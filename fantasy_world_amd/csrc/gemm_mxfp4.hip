@@ -410,19 +410,172 @@ __global__ __launch_bounds__(512, 2) void gemm_mxfp4_256_kernel(MxArgs p) {
     mx_finish<2>(p, smem + wave * 16384, acc, lane, m0 + grp * 128, n0 + wn * 64);
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows (up to 64): the weights are all there is to read, so the split is made for them.  A work-group takes 16 NB columns (W rows) and all
+// rows of A, its 8 waves a run of K each, v_mfma_scale_f32_16x16x128_f8f6f4 (lane l: row l & 15, block l >> 4 of four); a wave requests all
+// W of eight instructions before it multiplies, which keeps the whole matrix in flight across the chip.  The eight partial sums are added
+// in LDS, in wave order: no atomics, no workspace, the same bits every time.
+// FUSED (up to 16 rows): A is bf16 and the work-group quantises all of it into LDS, a block of 32 a lane, while its first W is on the way;
+// every work-group repeats that, which costs less than a launch and a round trip through memory.  LDS rows are padded by one 16-byte chunk,
+// so the fragment reads of 16 rows hit 16 different chunks.
+// ---------------------------------------------------------------------------------------------------------------
+#define FWX_MFMA16(A, B, C, SA, SB) __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( \
+    i32x8_t{(A)[0], (A)[1], (A)[2], (A)[3], 0, 0, 0, 0}, i32x8_t{(B)[0], (B)[1], (B)[2], (B)[3], 0, 0, 0, 0}, C, 4, 4, 0, SA, 0, SB)
+
+template <int MT, int NB, bool FUSED>
+__global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void gemm_mxfp4_rows_kernel(MxArgs p, int blocks) {
+    constexpr int UB = MT * NB == 1 ? 8 : 4;              // instructions (of 128 values of K) whose operands are requested together
+    __shared__ float red[8][MT * NB * 4][64];
+    extern __shared__ u32x4_t mx_rows[];                  // FUSED: codes [M][slabs * 8 + 1] chunks, then scale bytes [M][slabs * 8]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, h = lane >> 4;
+    const int n0 = blockIdx.x * 16 * NB;
+    const int units = p.slabs * 2, u0 = wave * units / 8, u1 = (wave + 1) * units / 8;
+    // rows past the end repeat the last one: their results are never stored
+    const uint8_t* wp[NB];
+    const uint8_t* swp[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int n = min(n0 + b * 16 + r, p.N - 1);
+        wp[b] = p.W + (int64_t)n * p.ldw + h * 16;
+        swp[b] = p.sw + (int64_t)(n >> 5) * p.slabs * 256 + (n & 31) * 8 + h;
+    }
+    const uint8_t* ap[MT];
+    const uint8_t* sap[MT];
+    const int chunks = p.slabs * 8;                       // 16-byte chunks = blocks of a padded row
+    uint8_t* smem_s = (uint8_t*)(mx_rows + p.M * (chunks + 1));
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int row = min(m * 16 + r, p.M - 1);
+        ap[m] = FUSED ? (const uint8_t*)(mx_rows + row * (chunks + 1) + h) : p.A + (int64_t)row * p.lda + h * 16;
+        sap[m] = FUSED ? smem_s + row * chunks + h : p.sa + (int64_t)(row >> 5) * p.slabs * 256 + (row & 31) * 8 + h;
+    }
+    f32x4_t acc[MT][NB];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[m][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    i32x4_t w[UB][NB], a[UB][MT];
+    int sw[UB][NB], sa[UB][MT];
+    auto load_w = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < UB; ++i)
+            if (u + i < u1) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    w[i][b] = *(const i32x4_t*)(wp[b] + (int64_t)(u + i) * 64);
+                    sw[i][b] = swp[b][(int64_t)((u + i) >> 1) * 256 + ((u + i) & 1) * 4];
+                }
+            }
+    };
+    load_w(u0);
+    if (FUSED) {
+        for (int i = threadIdx.x; i < p.M * chunks; i += 512) {
+            const int row = i / chunks, c = i - row * chunks;
+            u32x4_t x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = c < blocks ? *(const u32x4_t*)(p.A + (int64_t)row * p.lda + c * 64 + j * 16) : u32x4_t{0, 0, 0, 0};
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = max(top, mx_top8_bf16(x[j]));
+            const uint32_t byte = mx_scale_byte(top);
+            u32x4_t q;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[j] = mx_pack8_bf16(x[j], mx_scale_f32(byte));
+            mx_rows[row * (chunks + 1) + c] = q;
+            smem_s[i] = (uint8_t)byte;
+        }
+        __syncthreads();
+    }
+    for (int u = u0; u < u1; u += UB) {
+        if (u != u0) load_w(u);
+#pragma unroll
+        for (int i = 0; i < UB; ++i)
+            if (u + i < u1) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    a[i][m] = *(const i32x4_t*)(ap[m] + (int64_t)(u + i) * 64);
+                    sa[i][m] = FUSED ? sap[m][(u + i) * 4] : sap[m][(int64_t)((u + i) >> 1) * 256 + ((u + i) & 1) * 4];
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < UB; ++i)
+            if (u + i < u1) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) acc[m][b] = FWX_MFMA16(a[i][m], w[i][b], acc[m][b], sa[i][m], sw[i][b]);
+            }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) red[wave][(m * NB + b) * 4 + i][lane] = acc[m][b][i];
+    __syncthreads();
+    // lane l of a fragment holds column l & 15 of rows 4 (l >> 4) .. + 3
+    constexpr int COLS = 16 * NB, OUT = MT * 16 * COLS;
+#pragma unroll
+    for (int e0 = 0; e0 < OUT; e0 += 512) {
+        const int e = e0 + threadIdx.x;
+        if (OUT < 512 && e >= OUT) break;                 // whole waves: OUT is 256, or a multiple of 512
+        const int row = e / COLS, c = e % COLS, col = n0 + c;
+        const int slot = ((row >> 4) * NB + (c >> 4)) * 4 + (row & 3), at = ((row >> 2) & 3) * 16 + (c & 15);
+        float v = red[0][slot][at];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) v += red[k][slot][at];
+        const bool in = col < p.N, live = row < p.M;
+        if (p.bias && in) v += p.bias[col];
+        v = fw_apply_act(v, p.act);
+        if ((p.g1 || p.g0) && in) v = fw_affine(v, p.g1 ? p.g1[col] : 1.f, p.g0 ? p.g0[col] : 0.f);
+        if (p.res_dtype != FW_DT_NONE && in && live) {
+            const int64_t o = (int64_t)row * p.ldr + col;
+            v += p.res_dtype == FW_DT_F32 ? ((const float*)p.res)[o] : bf16_bits_to_f32(((const uint16_t*)p.res)[o]);
+        }
+        if (NB == 2 && p.out_dtype == FW_DT_MXFP4) {      // 32 lanes hold a block
+            const uint32_t b16 = in ? f32_to_bf16_bits(v) : 0;
+            uint32_t top = (b16 & 0x7fffu) << 16;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+            const uint32_t byte = mx_scale_byte(top);
+            uint32_t q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(0u, mx_pair(b16), mx_scale_f32(byte), 0) & 15u;
+            q <<= 4 * (c & 7);
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) q |= (uint32_t)__shfl_xor((int)q, o, 64);
+            if (live && (c & 7) == 0) *(uint32_t*)((uint8_t*)p.C + (int64_t)row * p.ldc + (col >> 1)) = q;
+            if (live && c == 0) p.cs[((int64_t)(row >> 5) * p.cslabs + (col >> 8)) * 256 + (row & 31) * 8 + ((col >> 5) & 7)] = (uint8_t)byte;
+        } else if (live && in) {
+            const int64_t o = (int64_t)row * p.ldc + col;
+            if (p.out_dtype == FW_DT_F32) ((float*)p.C)[o] = v;
+            else ((uint16_t*)p.C)[o] = f32_to_bf16_bits(v);
+        }
+    }
+}
+
+template <int MT, bool FUSED>
+int mx_launch_rows(const MxArgs& p, int n_cover, int blocks, hipStream_t st) {
+    const int lds = FUSED ? p.M * (p.slabs * 8 + 1) * 16 + p.M * p.slabs * 8 : 0;
+    if (p.out_dtype == FW_DT_MXFP4) hipLaunchKernelGGL((gemm_mxfp4_rows_kernel<MT, 2, FUSED>), dim3((unsigned)((n_cover + 31) / 32)), dim3(512), lds, st, p, blocks);
+    else hipLaunchKernelGGL((gemm_mxfp4_rows_kernel<MT, 1, FUSED>), dim3((unsigned)((n_cover + 15) / 16)), dim3(512), lds, st, p, blocks);
+    return (int)hipGetLastError();
+}
+
+// Rows that fw_linear_mxfp4 quantises inside the product: at most 16, in whole 16-byte accessible blocks, that take at most 48 KiB of LDS
+// (two work-groups of 8 waves a CU; 16 x 5120 takes 44)
+bool mx_rows_fused(const void* x, int64_t ldx, int M, int K) {
+    return M <= 16 && K > 0 && (K % 32) == 0 && (ldx % 8) == 0 && (((uintptr_t)x) & 15) == 0 && (int64_t)M * (mx_slabs(K) * 136 + 16) <= 48 * 1024;
+}
+
 }  // namespace
 
-extern "C" int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, const uint8_t* W, int64_t ldw, const uint8_t* sw,
-                             void* C, int64_t ldc, int out_dtype, uint8_t* cs, int M, int N, int K,
-                             const float* bias, int act, const float* g1, const float* g0,
-                             const void* res, int64_t ldr, int res_dtype, void* stream) {
-    if (M <= 0 || N <= 0) return 0;
-    const int slabs = mx_slabs(K);
-    if (!A || !sa || !W || !sw || !C || K <= 0 || lda < (int64_t)slabs * 128 || ldw < (int64_t)slabs * 128 || (lda % 16) || (ldw % 16) ||
-        lda >= (1 << 23) || ldw >= (1 << 23) || ((((uintptr_t)A) | ((uintptr_t)W)) & 15) || ((((uintptr_t)sa) | ((uintptr_t)sw)) & 3)) {
-        fw_set_error("fw_gemm_mxfp4: K > 0; A / W 16-byte aligned with roundup(K, 256) / 2 <= ld < 2^23, ld % 16 == 0; scales 4-byte aligned"); return FW_E_BADARG; }
+// Everything but A: the checks that fw_gemm_mxfp4 and fw_linear_mxfp4 share, and the arguments.  0, or the error code with its message set.
+static int mx_args(MxArgs& p, const uint8_t* W, int64_t ldw, const uint8_t* sw, void* C, int64_t ldc, int out_dtype, uint8_t* cs, int M, int N, int K,
+                   const float* bias, int act, const float* g1, const float* g0, const void* res, int64_t ldr, int res_dtype) {
+    const int slabs = mx_slabs(K), cslabs = mx_slabs(N);
+    if (!W || !sw || !C || K <= 0 || ldw < (int64_t)slabs * 128 || (ldw % 16) || ldw >= (1 << 23) || (((uintptr_t)W) & 15) || (((uintptr_t)sw) & 3)) {
+        fw_set_error("fw_gemm_mxfp4: K > 0; W 16-byte aligned with roundup(K, 256) / 2 <= ldw < 2^23, ldw % 16 == 0; scales 4-byte aligned"); return FW_E_BADARG; }
     if (act < FW_ACT_NONE || act > FW_ACT_SILU) { fw_set_error("fw_gemm_mxfp4: bad act"); return FW_E_BADARG; }
-    const int cslabs = mx_slabs(N);
     if (out_dtype == FW_DT_MXFP4) {
         if (!cs || ldc < (int64_t)cslabs * 128 || (ldc % 16) || (((uintptr_t)C) & 15) || (((uintptr_t)cs) & 3)) {
             fw_set_error("fw_gemm_mxfp4: MXFP4 output needs c_scale, C 16-byte aligned, ldc % 16 == 0 and ldc >= roundup(N, 256) / 2"); return FW_E_BADARG; }
@@ -431,16 +584,30 @@ extern "C" int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, c
     if (res_dtype != FW_DT_NONE && (!res || (res_dtype != FW_DT_BF16 && res_dtype != FW_DT_F32) || ldr < N || (((uintptr_t)res) & (res_dtype == FW_DT_F32 ? 3 : 1)))) {
         fw_set_error("fw_gemm_mxfp4: res_dtype set but res NULL, misaligned, of another type or ldr < N"); return FW_E_BADARG; }
     if ((((uintptr_t)bias) | ((uintptr_t)g1) | ((uintptr_t)g0)) & 3) { fw_set_error("fw_gemm_mxfp4: misaligned bias / g1 / g0"); return FW_E_BADARG; }
-    MxArgs p;
-    p.A = A; p.lda = lda; p.sa = sa; p.W = W; p.ldw = ldw; p.sw = sw; p.C = C; p.ldc = ldc; p.out_dtype = out_dtype; p.cs = cs;
+    p.W = W; p.ldw = ldw; p.sw = sw; p.C = C; p.ldc = ldc; p.out_dtype = out_dtype; p.cs = cs;
     p.M = M; p.N = N; p.slabs = slabs; p.bias = bias; p.act = act; p.g1 = g1; p.g0 = g0;
     p.res = res; p.ldr = ldr; p.res_dtype = res_dtype; p.cslabs = cslabs;
     // 16-byte accesses of 8 columns in the epilogue
     const int ce = out_dtype == FW_DT_F32 ? 4 : 8, re = res_dtype == FW_DT_F32 ? 4 : 8;
     p.vec = (N % 8) == 0 && (out_dtype == FW_DT_MXFP4 || ((ldc % ce) == 0 && (((uintptr_t)C) & 15) == 0)) &&
             (res_dtype == FW_DT_NONE || ((ldr % re) == 0 && (((uintptr_t)res) & 15) == 0));
+    return 0;
+}
+
+extern "C" int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, const uint8_t* W, int64_t ldw, const uint8_t* sw,
+                             void* C, int64_t ldc, int out_dtype, uint8_t* cs, int M, int N, int K,
+                             const float* bias, int act, const float* g1, const float* g0,
+                             const void* res, int64_t ldr, int res_dtype, void* stream) {
+    if (M <= 0 || N <= 0) return 0;
+    MxArgs p;
+    if (const int rc = mx_args(p, W, ldw, sw, C, ldc, out_dtype, cs, M, N, K, bias, act, g1, g0, res, ldr, res_dtype)) return rc;
+    const int slabs = p.slabs, cslabs = p.cslabs;
+    if (!A || !sa || lda < (int64_t)slabs * 128 || (lda % 16) || lda >= (1 << 23) || (((uintptr_t)A) & 15) || (((uintptr_t)sa) & 3)) {
+        fw_set_error("fw_gemm_mxfp4: A 16-byte aligned with roundup(K, 256) / 2 <= lda < 2^23, lda % 16 == 0; scales 4-byte aligned"); return FW_E_BADARG; }
+    p.A = A; p.lda = lda; p.sa = sa;
     const int n_cover = out_dtype == FW_DT_MXFP4 ? cslabs * MX_SLAB : N;       // the padding of a quantised row is written too
     hipStream_t st = (hipStream_t)stream;
+    if (M <= 64) return M <= 16 ? mx_launch_rows<1, false>(p, n_cover, 0, st) : M <= 32 ? mx_launch_rows<2, false>(p, n_cover, 0, st) : mx_launch_rows<4, false>(p, n_cover, 0, st);
     // 256 x 256 tiles from two full rounds' worth of rows and columns on; below, and for a tail of at most 128 rows past the last full
     // tile (a whole extra round of 256-row tiles otherwise), the 128 x 128 kernel.  Both add the same instructions in the same order per
     // output element: a row's bits do not depend on the kernel that computes it.
@@ -467,4 +634,34 @@ extern "C" int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, c
     if (nwg > 0x7fffffff) { fw_set_error("fw_gemm_mxfp4: grid too large"); return FW_E_BADARG; }
     hipLaunchKernelGGL(gemm_mxfp4_128_kernel, dim3((unsigned)nwg), dim3(256), 0, st, p);
     return (int)hipGetLastError();
+}
+
+extern "C" int64_t fw_linear_mxfp4_workspace_bytes(int M, int K) {
+    if (M <= 0 || K <= 0) return 0;
+    const int64_t slabs = mx_slabs(K);
+    return (int64_t)M * slabs * 128 + (int64_t)((M + 31) / 32) * slabs * 256;
+}
+
+extern "C" int fw_linear_mxfp4(const uint16_t* x, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* sw,
+                               void* C, int64_t ldc, int out_dtype, uint8_t* cs, int M, int N, int K,
+                               const float* bias, int act, const float* g1, const float* g0,
+                               const void* res, int64_t ldr, int res_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (!x || ldx < K || (((uintptr_t)x) & 1)) { fw_set_error("fw_linear_mxfp4: bf16 x with ldx >= K required"); return FW_E_BADARG; }
+    if (mx_rows_fused(x, ldx, M, K)) {
+        MxArgs p;
+        if (const int rc = mx_args(p, W, ldw, sw, C, ldc, out_dtype, cs, M, N, K, bias, act, g1, g0, res, ldr, res_dtype)) return rc;
+        p.A = (const uint8_t*)x; p.lda = ldx * 2; p.sa = nullptr;
+        return mx_launch_rows<1, true>(p, out_dtype == FW_DT_MXFP4 ? p.cslabs * MX_SLAB : N, K / 32, (hipStream_t)stream);
+    }
+    if (!workspace || workspace_bytes < fw_linear_mxfp4_workspace_bytes(M, K) || (((uintptr_t)workspace) & 15)) {
+        fw_set_error("fw_linear_mxfp4: a 16-byte aligned workspace of fw_linear_mxfp4_workspace_bytes(M, K) required"); return FW_E_BADARG; }
+    const int64_t lda = (int64_t)mx_slabs(K) * 128;
+    uint8_t* q = (uint8_t*)workspace;
+    uint8_t* s = q + (int64_t)M * lda;
+    // the product's arguments first: nothing is launched for a call that is refused
+    MxArgs p;
+    if (const int rc = mx_args(p, W, ldw, sw, C, ldc, out_dtype, cs, M, N, K, bias, act, g1, g0, res, ldr, res_dtype)) return rc;
+    if (const int rc = fw_mxfp4_quant_rows(x, ldx, FW_DT_BF16, q, lda, s, M, K, stream)) return rc;
+    return fw_gemm_mxfp4(q, lda, s, W, ldw, sw, C, ldc, out_dtype, cs, M, N, K, bias, act, g1, g0, res, ldr, res_dtype, stream);
 }

@@ -32,7 +32,7 @@ SYMBOLS = [
     "fw_row_sumsq", "fw_qk_prep_tp", "fw_residual_add", "fw_cfg_euler_step",
     "fw_qk_prep_fp8", "fw_v_transpose_e4m3", "fw_row_absmax", "fw_fp8_quant_rows_amax", "fw_modulation_tables",
     "fw_layernorm_mod_split",
-    "fw_mxfp4_quant_rows", "fw_mxfp4_dequant_rows", "fw_gemm_mxfp4", "fw_residual_norm",
+    "fw_mxfp4_quant_rows", "fw_mxfp4_dequant_rows", "fw_gemm_mxfp4", "fw_linear_mxfp4", "fw_linear_mxfp4_workspace_bytes", "fw_residual_norm",
 ]
 
 _lib = None
@@ -105,12 +105,15 @@ def load_library(path: str = LIB_PATH, cache: bool = True):
         "fw_mxfp4_quant_rows": [vp, i64, i32, vp, i64, vp, i32, i32, vp],
         "fw_mxfp4_dequant_rows": [vp, i64, vp, vp, i64, i32, i32, i32, vp],
         "fw_gemm_mxfp4": [vp, i64, vp, vp, i64, vp, vp, i64, i32, vp, i32, i32, i32, vp, i32, vp, vp, vp, i64, i32, vp],
+        "fw_linear_mxfp4": [vp, i64, vp, i64, vp, vp, i64, i32, vp, i32, i32, i32, vp, i32, vp, vp, vp, i64, i32, vp, i64, vp],
         "fw_residual_norm": [vp, i64, vp, i64, i32, vp, i64, i32, vp, vp, vp, i32, vp, i32, vp, vp, vp, vp, f32, vp, i64, i32, vp, i32, i32, i32, vp],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)
         fn.restype = i32
         fn.argtypes = args
+    lib.fw_linear_mxfp4_workspace_bytes.restype = i64
+    lib.fw_linear_mxfp4_workspace_bytes.argtypes = [i32, i32]
     lib.fw_attention_workspace_bytes.restype = i64
     lib.fw_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
     if lib.fw_abi_version() != 12:
@@ -152,18 +155,46 @@ class Linear:
 
 class MXFP4Rows:
     """A matrix held as MXFP4 rows (include/fw_mi355x.h): codes q uint8 [M, Kp / 2], scales s uint8 [ceil(M / 32), Kp / 256, 32, 8], Kp = K rounded
-    up to 256."""
-    __slots__ = ("q", "s", "M", "K")
+    up to 256.  Padding past K: codes zero, scale bytes anything but 0xff."""
+    __slots__ = ("_buf", "_q", "_s", "M", "K", "qp", "sp", "ldq")
+    mxfp4 = True
 
     def __init__(self, q, s, K):
-        if q.dtype != torch.uint8 or q.dim() != 2 or q.stride(1) != 1 or K <= 0 or q.shape[1] != (K + 255) // 256 * 128:
+        slabs = (K + 255) // 256
+        if q.dtype is not torch.uint8 or q.dim() != 2 or q.stride(1) != 1 or K <= 0 or q.shape[1] != slabs * 128:
             raise ValueError(f"MXFP4 codes: uint8 [M, roundup(K, 256) / 2] with contiguous rows expected, got {q.dtype} {tuple(q.shape)} for K = {K}")
-        want = ((q.shape[0] + 31) // 32, q.shape[1] // 128, 32, 8)
-        if s.dtype != torch.uint8 or tuple(s.shape) != want or not s.is_contiguous():
-            raise ValueError(f"MXFP4 scales: contiguous uint8 {want} expected, got {s.dtype} {tuple(s.shape)}")
-        if q.device != s.device:
+        M = q.shape[0]
+        if s.dtype is not torch.uint8 or s.shape != ((M + 31) // 32, slabs, 32, 8) or not s.is_contiguous():
+            raise ValueError(f"MXFP4 scales: contiguous uint8 {((M + 31) // 32, slabs, 32, 8)} expected, got {s.dtype} {tuple(s.shape)}")
+        if q.get_device() != s.get_device():
             raise ValueError(f"MXFP4 codes on {q.device}, scales on {s.device}")
-        self.q, self.s, self.M, self.K = q, s, q.shape[0], K
+        self._buf, self._q, self._s, self.M, self.K = q, q, s, M, K
+        self.qp, self.sp, self.ldq = q.data_ptr(), s.data_ptr(), q.stride(0)
+
+    @classmethod
+    def _unwritten(cls, M, K, device):
+        """Codes and scales in one allocation, for a kernel to fill."""
+        self = cls.__new__(cls)
+        slabs = (K + 255) // 256
+        self.ldq = slabs * 128
+        self._buf = torch.empty(M * self.ldq + (M + 31) // 32 * slabs * 256, dtype=torch.uint8, device=device)
+        self._q = self._s = None
+        self.M, self.K = M, K
+        self.qp = self._buf.data_ptr()
+        self.sp = self.qp + M * self.ldq
+        return self
+
+    @property
+    def q(self):
+        if self._q is None:
+            self._q = self._buf[:self.M * self.ldq].view(self.M, self.ldq)
+        return self._q
+
+    @property
+    def s(self):
+        if self._s is None:
+            self._s = self._buf[self.M * self.ldq:].view((self.M + 31) // 32, self.ldq // 128, 32, 8)
+        return self._s
 
     @property
     def shape(self):
@@ -173,19 +204,18 @@ class MXFP4Rows:
 class LinearMXFP4(MXFP4Rows):
     """Pre-packed nn.Linear with MXFP4 weights [N, K] and an fp32 bias [N]; HipOps.linear quantises the activation rows (or takes them as
     MXFP4Rows)."""
-    __slots__ = ("b",)
+    __slots__ = ("b", "N")
     fp8 = False
-    mxfp4 = True
 
     def __init__(self, q, s, b, K):
         super().__init__(q, s, K)
-        if b is not None and (b.dtype != torch.float32 or b.shape != (self.M,) or not b.is_contiguous()):
-            raise ValueError(f"bias: contiguous fp32 [{self.M}] expected, got {b.dtype} {tuple(b.shape)}")
-        self.b = b
+        self._bias(b)
 
-    @property
-    def N(self):
-        return self.M
+    def _bias(self, b):
+        if b is not None and (b.dtype is not torch.float32 or b.shape != (self.M,) or not b.is_contiguous() or b.get_device() != self._buf.get_device()):
+            raise ValueError(f"bias: contiguous fp32 [{self.M}] on the weights' device expected, got {b.dtype} {tuple(b.shape)} on {b.device}")
+        self.b, self.N = b, self.M
+        return self
 
 
 class LinearF32:
@@ -716,29 +746,45 @@ class HipOps:
         return out
 
     # ---- MXFP4 linear (include/fw_mi355x.h; no reference semantics) ------------------------------------------------------------------
-    def _mxfp4_empty(self, M, K):
-        """Unwritten MXFP4 rows on this device: (codes [M, Kp / 2], scales)."""
-        slabs = (K + 255) // 256
-        return (torch.empty(M, slabs * 128, dtype=torch.uint8, device=self.device),
-                torch.empty((M + 31) // 32, slabs, 32, 8, dtype=torch.uint8, device=self.device))
+    def _enter(self, *tensors):
+        """The current stream, for a call whose tensors all lie on the current device (and on the one this object is bound to)."""
+        dev = torch.cuda.current_device()
+        if self.device.index is not None and dev != self.device.index:
+            raise RuntimeError(f"HipOps bound to {self.device} but the current HIP device is {dev}: call torch.cuda.set_device(...) (one process per GPU)")
+        for t in tensors:
+            if t is not None and t.get_device() != dev:
+                raise RuntimeError(f"tensor on {t.device} passed to HipOps on cuda:{dev}")
+        return torch._C._cuda_getCurrentRawStream(dev)
+
+    @staticmethod
+    def _rows(name, t, *dtypes):
+        """t [rows, width], one of dtypes, contiguous inside a row; -> its row stride (at least the width, where there is at most one row)."""
+        if t.dim() != 2 or t.dtype not in dtypes or t.shape[1] < 1 or (t.stride(1) != 1 and t.shape[1] > 1):
+            raise ValueError(f"{name}: rows of {dtypes} expected, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+        ld = t.stride(0)
+        return ld if ld >= t.shape[1] else HipOps._short(name, t)
+
+    @staticmethod
+    def _short(name, t):
+        if t.shape[0] > 1:
+            raise ValueError(f"{name}: rows overlap, shape {tuple(t.shape)} with strides {t.stride()}")
+        return t.shape[1]
 
     def quantize_mxfp4_rows(self, x):
         """x bf16 / fp32 [M, K] (rows may be strided, any K) -> MXFP4Rows."""
-        if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or x.shape[1] < 1:
-            raise ValueError(f"bf16 / fp32 rows expected, got {x.dtype} {tuple(x.shape)} with strides {x.stride()}")
-        self._check_dev(x)
+        ldx = self._rows("x", x, torch.bfloat16, torch.float32)
+        st = self._enter(x)
         M, K = x.shape
-        q, s = self._mxfp4_empty(M, K)
-        _check(self.lib.fw_mxfp4_quant_rows(x.data_ptr(), max(x.stride(0), K), _dt(x), q.data_ptr(), q.stride(0), s.data_ptr(), M, K, self._stream()),
+        mx = MXFP4Rows._unwritten(M, K, x.device)
+        _check(self.lib.fw_mxfp4_quant_rows(x.data_ptr(), ldx, FW_DT_BF16 if x.dtype is torch.bfloat16 else FW_DT_F32, mx.qp, mx.ldq, mx.sp, M, K, st),
                "fw_mxfp4_quant_rows")
-        return MXFP4Rows(q, s, K)
+        return mx
 
     def dequantize_mxfp4_rows(self, mx, dtype=torch.bfloat16):
         """MXFP4Rows -> [M, K] in bf16 or fp32 (exact in both)."""
-        self._check_dev(mx.q, mx.s)
-        y = torch.empty(mx.M, mx.K, dtype=dtype, device=self.device)
-        _check(self.lib.fw_mxfp4_dequant_rows(mx.q.data_ptr(), mx.q.stride(0), mx.s.data_ptr(), y.data_ptr(), mx.K, _dt(y), mx.M, mx.K, self._stream()),
-               "fw_mxfp4_dequant_rows")
+        st = self._enter(mx._buf, mx._s)
+        y = torch.empty((mx.M, mx.K), dtype=dtype, device=mx._buf.device)
+        _check(self.lib.fw_mxfp4_dequant_rows(mx.qp, mx.ldq, mx.sp, y.data_ptr(), mx.K, _dt(y), mx.M, mx.K, st), "fw_mxfp4_dequant_rows")
         return y
 
     def pack_linear_mxfp4(self, w, b):
@@ -749,43 +795,67 @@ class HipOps:
 
     def linear_from_mxfp4(self, q, s, b, K):
         """A linear whose weights are MXFP4 rows already (q, s as in MXFP4Rows; b fp32 [N] or None), without a copy."""
-        self._check_dev(q, s, b)
-        return LinearMXFP4(q, s, b, K)
+        lin = LinearMXFP4(q, s, b, K)
+        self._enter(q)
+        return lin
 
     def _linear_mxfp4(self, x, lin, act=None, g1=None, g0=None, res=None, out_f32=False, out=None, out_mxfp4=False):
         """bf16 rows (quantised here) or MXFP4Rows x -> epilogue(x W^T): bf16, fp32 or MXFP4Rows."""
-        if not isinstance(x, MXFP4Rows):
-            if not torch.is_tensor(x) or x.dtype != torch.bfloat16:
-                raise ValueError(f"an MXFP4 linear takes bf16 rows or MXFP4Rows, got {getattr(x, 'dtype', type(x))}")
-            x = self.quantize_mxfp4_rows(x)
-        if x.K != lin.K:
-            raise ValueError(f"x has K = {x.K}, the linear K = {lin.K}")
-        self._check_dev(x.q, x.s, lin.q, lin.s, lin.b, g1, g0, res, out)
-        M, N = x.M, lin.N
-        for name, v in (("g1", g1), ("g0", g0)):
-            if v is not None and (v.dtype != torch.float32 or v.numel() != N or not v.is_contiguous()):
-                raise ValueError(f"{name}: contiguous fp32 [{N}] expected, got {v.dtype} {tuple(v.shape)}")
-        if res is not None and (res.shape != (M, N) or (N > 1 and res.stride(1) != 1)):
-            raise ValueError(f"res: [{M}, {N}] with contiguous rows expected, got {tuple(res.shape)} with strides {res.stride()}")
-        cs = None
+        N = lin.N
+        ready = isinstance(x, MXFP4Rows)
+        if ready:
+            M, K, xt = x.M, x.K, x._buf
+        else:
+            if not torch.is_tensor(x):
+                raise ValueError(f"an MXFP4 linear takes bf16 rows or MXFP4Rows, got {type(x)}")
+            ldx = self._rows("x", x, torch.bfloat16)
+            (M, K), xt = x.shape, x
+        if K != lin.K:
+            raise ValueError(f"x has K = {K}, the linear K = {lin.K}")
+        st = self._enter(xt, lin._buf, g1, g0, res, out)
+        g1p = g0p = resp = ldr = 0
+        rdt = FW_DT_NONE
+        if g1 is not None or g0 is not None:
+            for name, v in (("g1", g1), ("g0", g0)):
+                if v is not None and (v.dtype is not torch.float32 or v.numel() != N or not v.is_contiguous()):
+                    raise ValueError(f"{name}: contiguous fp32 [{N}] expected, got {v.dtype} {tuple(v.shape)}")
+            g1p, g0p = _ptr(g1), _ptr(g0)
+        if res is not None:
+            ldr = self._rows("res", res, torch.bfloat16, torch.float32)
+            if res.shape != (M, N):
+                raise ValueError(f"res: [{M}, {N}] expected, got {tuple(res.shape)}")
+            resp, rdt = res.data_ptr(), _dt(res)
         if out_mxfp4:
             if out is not None or out_f32:
                 raise ValueError("out_mxfp4 allocates its own output and excludes out_f32")
-            c, cs = self._mxfp4_empty(M, N)
-            ldc, odt = c.stride(0), FW_DT_MXFP4
+            y = MXFP4Rows._unwritten(M, N, xt.device)
+            yp, ldc, odt, csp = y.qp, y.ldq, FW_DT_MXFP4, y.sp
         else:
-            c = out if out is not None else torch.empty(M, N, dtype=torch.float32 if out_f32 else torch.bfloat16, device=self.device)
-            if c.shape != (M, N) or (N > 1 and c.stride(1) != 1):
-                raise ValueError(f"out: [{M}, {N}] with contiguous rows expected, got {tuple(c.shape)} with strides {c.stride()}")
-            ldc, odt = max(c.stride(0), N), _dt(c)
+            y = out
+            if out is None:
+                y, ldc, odt = torch.empty((M, N), dtype=torch.float32 if out_f32 else torch.bfloat16, device=xt.device), N, FW_DT_F32 if out_f32 else FW_DT_BF16
+            else:
+                ldc, odt = self._rows("out", out, torch.bfloat16, torch.float32), _dt(out)
+                if out.shape != (M, N):
+                    raise ValueError(f"out: [{M}, {N}] expected, got {tuple(out.shape)}")
+            yp, csp = y.data_ptr(), 0
         tok = None if self._timing is None else self._time_begin(
-            dict(kind="linear", M=M, N=N, K=x.K, res=res is not None, out_f32=odt == FW_DT_F32, act=act, mxfp4=True))
-        _check(self.lib.fw_gemm_mxfp4(
-            x.q.data_ptr(), x.q.stride(0), x.s.data_ptr(), lin.q.data_ptr(), lin.q.stride(0), lin.s.data_ptr(), c.data_ptr(), ldc, odt, _ptr(cs),
-            M, N, x.K, _ptr(lin.b), ACT[act], _ptr(g1), _ptr(g0), _ptr(res), 0 if res is None else max(res.stride(0), N),
-            FW_DT_NONE if res is None else _dt(res), self._stream()), "fw_gemm_mxfp4")
+            dict(kind="linear", M=M, N=N, K=K, res=res is not None, out_f32=odt == FW_DT_F32, act=act, mxfp4=True))
+        bp = 0 if lin.b is None else lin.b.data_ptr()
+        if ready:
+            _check(self.lib.fw_gemm_mxfp4(x.qp, x.ldq, x.sp, lin.qp, lin.ldq, lin.sp, yp, ldc, odt, csp, M, N, K, bp, ACT[act], g1p, g0p, resp, ldr, rdt, st),
+                   "fw_gemm_mxfp4")
+        else:
+            # scratch for the quantised rows (PyTorch owns the memory); few whole-block rows are quantised inside the product
+            ws, wsp, wsn, slabs = None, 0, 0, (K + 255) // 256
+            if M > 16 or K % 32 or ldx % 8 or x.data_ptr() % 16 or M * (slabs * 136 + 16) > 48 * 1024:
+                wsn = M * slabs * 128 + (M + 31) // 32 * slabs * 256            # fw_linear_mxfp4_workspace_bytes
+                ws = torch.empty(wsn, dtype=torch.uint8, device=xt.device)
+                wsp = ws.data_ptr()
+            _check(self.lib.fw_linear_mxfp4(x.data_ptr(), ldx, lin.qp, lin.ldq, lin.sp, yp, ldc, odt, csp, M, N, K, bp, ACT[act], g1p, g0p, resp, ldr, rdt,
+                                            wsp, wsn, st), "fw_linear_mxfp4")
         self._time_end(tok)
-        return MXFP4Rows(c, cs, N) if out_mxfp4 else c
+        return y
 
     def linear_mxfp4(self, x, lin, **kw):
         """linear() for callers that want a refusal when `lin` is not an MXFP4 linear."""
@@ -798,45 +868,53 @@ class HipOps:
                       norm="layer", eps=1e-6, x_out=None, out="bf16"):
         """x' = x + [post norm](y + bias) * g1 + g0, written to x_out (default: x, in place); -> h = norm(x') * w + b, * (1 + scale) + shift, as
         bf16 rows or (out="mxfp4") MXFP4Rows.  y None: h alone.  x, x_out [rows, C] fp32 or bf16, y fp32 or bf16; bias / post_w / w / b [C];
-        g1 / g0 / scale / shift [C] or [groups, C] with rows % groups == 0: equal runs of rows share a vector.  post: None, "layer" or "rms"
+        g1 / g0 / scale / shift [C], or all of them [groups, C] with rows % groups == 0: equal runs of rows share a vector.  post: None, "layer" or "rms"
         (post_w only with it); norm: "layer" or "rms" (b only with w)."""
-        if x.dim() != 2 or x.dtype not in (torch.float32, torch.bfloat16) or (x.shape[1] > 1 and x.stride(1) != 1) or x.shape[1] < 1:
-            raise ValueError(f"x: fp32 / bf16 rows expected, got {x.dtype} {tuple(x.shape)} with strides {x.stride()}")
+        ldx = self._rows("x", x, torch.float32, torch.bfloat16)
         if out not in ("bf16", "mxfp4") or norm not in ("layer", "rms") or post not in RNORM:
             raise ValueError(f"out: 'bf16' | 'mxfp4', norm: 'layer' | 'rms', post: None | 'layer' | 'rms'; got {out!r}, {norm!r}, {post!r}")
         rows, C = x.shape
+        yp = xop = ldy = ldxo = 0
+        ydt, post = FW_DT_NONE, RNORM[post]
         if y is None:
             bias = g1 = g0 = post_w = x_out = None
-            post = None
+            post = 0
         else:
-            x_out = x if x_out is None else x_out
-            for name, v in (("y", y), ("x_out", x_out)):
-                if v.shape != x.shape or (C > 1 and v.stride(1) != 1) or (name == "x_out" and v.dtype != x.dtype):
-                    raise ValueError(f"{name}: rows of x's shape expected, got {v.dtype} {tuple(v.shape)} with strides {v.stride()}")
-        groups = 1
-        for name, v in (("g1", g1), ("g0", g0), ("scale", scale), ("shift", shift)):
-            if v is not None and v.dim() == 2 and v.shape[0] > 1:
-                if groups not in (1, v.shape[0]) or rows % v.shape[0]:
-                    raise ValueError(f"{name}: {v.shape[0]} vectors for {rows} rows in {groups} group(s)")
-                groups = v.shape[0]
-        for name, v, n in (("bias", bias, 1), ("post_w", post_w, 1), ("w", w, 1), ("b", b, 1), ("g1", g1, groups), ("g0", g0, groups),
-                           ("scale", scale, groups), ("shift", shift, groups)):
-            if v is not None and (v.dtype != torch.float32 or not v.is_contiguous() or v.numel() != n * C or v.shape[-1] != C):
-                raise ValueError(f"{name}: contiguous fp32 [{C}]" + (f" or [{n}, {C}]" if n > 1 else "") + f" expected, got {v.dtype} {tuple(v.shape)}")
-        if post in (None, "none"):
-            post_w = None
-        self._check_dev(x, y, bias, g1, g0, post_w, w, b, scale, shift, x_out)
-        hs = None
-        if out == "mxfp4":
-            h, hs = self._mxfp4_empty(rows, C)
+            ldy, yp, ydt = self._rows("y", y, torch.float32, torch.bfloat16), y.data_ptr(), _dt(y)
+            if x_out is None:
+                x_out, ldxo = x, ldx
+            else:
+                ldxo = self._rows("x_out", x_out, x.dtype)
+            xop = x_out.data_ptr()
+            if y.shape != x.shape or x_out.shape != x.shape:
+                raise ValueError(f"y, x_out: x's shape {tuple(x.shape)} expected, got {tuple(y.shape)}, {tuple(x_out.shape)}")
+            if not post:
+                post_w = None
+        groups, ptrs = 0, []
+        for name, v, many in (("bias", bias, False), ("g1", g1, True), ("g0", g0, True), ("post_w", post_w, False), ("w", w, False), ("b", b, False),
+                              ("scale", scale, True), ("shift", shift, True)):
+            if v is None:
+                ptrs.append(0)
+                continue
+            n = v.numel() // C
+            if v.dtype is not torch.float32 or v.shape[-1:] != (C,) or not v.is_contiguous() or n < 1 or (n > 1 and not many):
+                raise ValueError(f"{name}: contiguous fp32 [{C}]" + (f" or [groups, {C}]" if many else "") + f" expected, got {v.dtype} {tuple(v.shape)}")
+            if many and n != groups:
+                if groups or rows % n:
+                    raise ValueError(f"{name}: {n} vectors for {rows} rows; g1, g0, scale and shift alike in number, a divisor of the rows, expected")
+                groups = n
+            ptrs.append(v.data_ptr())
+        st = self._enter(x, y, x_out, bias, g1, g0, post_w, w, b, scale, shift)
+        mx = MXFP4Rows._unwritten(rows, C, x.device) if out == "mxfp4" else None
+        if mx is None:
+            h = torch.empty((rows, C), dtype=torch.bfloat16, device=x.device)
+            hp, ldh, hdt, hsp = h.data_ptr(), C, FW_DT_BF16, 0
         else:
-            h = torch.empty(rows, C, dtype=torch.bfloat16, device=self.device)
+            h, hp, ldh, hdt, hsp = mx, mx.qp, mx.ldq, FW_DT_MXFP4, mx.sp
         _check(self.lib.fw_residual_norm(
-            x.data_ptr(), max(x.stride(0), C), _ptr(x_out), 0 if x_out is None else max(x_out.stride(0), C), _dt(x),
-            _ptr(y), 0 if y is None else max(y.stride(0), C), FW_DT_NONE if y is None else _dt(y), _ptr(bias), _ptr(g1), _ptr(g0), RNORM[post], _ptr(post_w),
-            RNORM[norm], _ptr(w), _ptr(b), _ptr(scale), _ptr(shift), float(eps), h.data_ptr(), h.stride(0), FW_DT_MXFP4 if hs is not None else FW_DT_BF16,
-            _ptr(hs), rows, C, max(1, rows // groups), self._stream()), "fw_residual_norm")
-        return MXFP4Rows(h, hs, C) if hs is not None else h
+            x.data_ptr(), ldx, xop, ldxo, _dt(x), yp, ldy, ydt, ptrs[0], ptrs[1], ptrs[2], post, ptrs[3], RNORM[norm], ptrs[4], ptrs[5], ptrs[6], ptrs[7], eps,
+            hp, ldh, hdt, hsp, rows, C, max(1, rows // (groups or 1)), st), "fw_residual_norm")
+        return h
 
     # ---- fp8 attention (hd 128; parity unpinned: no reference semantics, see include/fw_mi355x.h) ---------------------------
     FP8_Q_EXP = 3      # Q8 holds q * softmax_scale * log2(e) * 2^3

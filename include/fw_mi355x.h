@@ -462,7 +462,7 @@ int fw_gemm_fp8(const uint8_t* A, int64_t lda, const uint8_t* W, int64_t ldw, co
  *   value: e2m1(v / scale), to nearest, ties to the even code; values above 6 scales saturate.
  * Storage ("MXFP4 rows", M x K): codes q [M][ldq] bytes, two values a byte with the first in the low half, K padded with zeros to
  *   Kp = roundup(K, 256): ldq >= Kp / 2, ldq % 16 == 0, q 16-byte aligned; scales s [ceil(M / 32)][Kp / 256][32][8] bytes, contiguous, 4-byte
- *   aligned: s[r / 32][k / 256][r % 32][k / 32 % 8].  Scale bytes of rows past M inside the last group of 32 are not read as values.
+ *   aligned: s[r / 32][k / 256][r % 32][k / 32 % 8].  Scale bytes of the padding past K are not 0xff; those of rows past M are not read as values.
  * ------------------------------------------------------------------------------------------------------------- */
 
 /* x [M][K] (bf16 or f32, ldx elements, any K and alignment of the element type) -> MXFP4 rows.  8 values per access where K % 8 == 0 and
@@ -481,6 +481,16 @@ int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, const uint8_
                   void* C, int64_t ldc, int out_dtype, uint8_t* cs, int M, int N, int K,
                   const float* bias, int act, const float* g1, const float* g0,
                   const void* res, int64_t ldr, int res_dtype, void* stream);
+
+/* The whole linear from bf16 rows: x [M][K] (ldx elements, any alignment of the element type) is quantised into the workspace and multiplied --
+ * or, up to 16 rows with K % 32 == 0, 16-byte aligned rows and M (roundup(K, 256) 17 / 32 + 16) <= 48 KiB, quantised inside the product in one
+ * launch, which reads no workspace (NULL, 0).  The rest as fw_gemm_mxfp4.  workspace: fw_linear_mxfp4_workspace_bytes(M, K) bytes, 16-byte
+ * aligned, the caller's until the call's work is done on `stream`. */
+int64_t fw_linear_mxfp4_workspace_bytes(int M, int K);
+int fw_linear_mxfp4(const uint16_t* x, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* sw,
+                    void* C, int64_t ldc, int out_dtype, uint8_t* cs, int M, int N, int K,
+                    const float* bias, int act, const float* g1, const float* g0,
+                    const void* res, int64_t ldr, int res_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The seam between two halves of a block in one pass: the gated residual update that ends one half and the norm that opens the next.
  *   t  = y + bias;  post: t = norm_post(t) * post_w;  x' = x + t * g1 + g0  (written to x_out, which may be x);
