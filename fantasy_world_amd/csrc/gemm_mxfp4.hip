@@ -31,6 +31,9 @@ struct MxArgs {
     i32x8_t{(A)[0], (A)[1], (A)[2], (A)[3], 0, 0, 0, 0}, i32x8_t{(B)[0], (B)[1], (B)[2], (B)[3], 0, 0, 0, 0}, C, 4, 4, J, SA, J, SB)
 #define FWX_BLDS16(rs, voff, soff, ldsptr) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, FW_LDS_PTR(ldsptr), 16, voff, soff, 0, 0)
 
+#define FWX_BARRIER() do { __builtin_amdgcn_sched_barrier(0); asm volatile("s_barrier" ::: "memory"); __builtin_amdgcn_sched_barrier(0); } while (0)
+template <int N> __device__ __forceinline__ void mx_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
 // descriptor over the rows from `base` on: an access past `bytes` reads zeros (a tile that lies in a quantised row's padding has no rows at all)
 __device__ __forceinline__ auto mx_rsrc(const uint8_t* base, long long bytes) {
     return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(unsigned)(bytes > 0xffffffffLL ? 0xffffffffLL : bytes < 0 ? 0 : bytes), 0x00020000);
@@ -48,7 +51,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& p, int& tm, int& tn) {
     tn = in_g / gsz;
 }
 
-// Epilogue of NQ quadrants (64 x 64 each, stacked along M) of a wave: accumulators -> LDS (16 KiB of the wave's own) -> rows -> bias,
+// Epilogue of NQ quadrants (32 RBK x 64 each, stacked along M) of a wave: accumulators -> LDS (16 KiB of the wave's own) -> rows -> bias,
 // activation, per-column affine, residual, store.  A lane owns 8 consecutive columns of a row, 8 rows per step: 16-byte accesses in bf16,
 // and with MXFP4 output a block of 32 columns is the 4 lanes of a quad.
 // LDS image: 16-byte chunk c of row r lies at (c >> 1) + 8 ((c ^ r) & 1) of the row's 16: the 16 lanes of a read (chunk 2q or 2q + 1 of two
@@ -56,7 +59,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& p, int& tm, int& tn) {
 // ACT, RES < 0: decided per element at run time.  VEC: every row of C and of the residual is 16-byte accessible and N % 8 == 0.
 // With a residual the 64 rows' loads are all in flight before the transpose, and the next quadrant's are issued as registers free up:
 // read one step at a time they cost a memory latency each (32 us per 256 x 256 tile with an fp32 residual, against 32 us of main loop).
-template <int ACT, int RES, bool VEC, int NQ, typename Acc>
+template <int ACT, int RES, bool VEC, int RBK, int NQ, typename Acc>
 __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Acc& acc, int lane, int m0, int n0) {
     const int fi = lane & 31, hi = lane >> 5, q = lane & 7, rl = lane >> 3;
     const int col = n0 + q * 8;
@@ -70,7 +73,8 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
         g1[j] = p.g1 && col + j < p.N ? p.g1[col + j] : 1.f;
         g0[j] = p.g0 && col + j < p.N ? p.g0[col + j] : 0.f;
     }
-    u32x4_t rv[8][RES == FW_DT_F32 ? 2 : 1];
+    constexpr int IT = 4 * RBK;                           // steps of 8 rows
+    u32x4_t rv[IT][RES == FW_DT_F32 ? 2 : 1];
     auto load_res = [&](int it, int row) __attribute__((always_inline)) {
         if (VEC && RES > 0 && in && row < p.M) {
             const char* r = (const char*)p.res + ((int64_t)row * p.ldr + col) * (RES == FW_DT_F32 ? 4 : 2);
@@ -80,7 +84,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
     };
     if (VEC && RES > 0) {
 #pragma unroll
-        for (int it = 0; it < 8; ++it) load_res(it, m0 + it * 8 + rl);
+        for (int it = 0; it < IT; ++it) load_res(it, m0 + it * 8 + rl);
     }
     auto quadrant = [&](auto q_tag) __attribute__((always_inline)) {
         constexpr int Q = decltype(q_tag)::value;
@@ -88,16 +92,16 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
         const int c = fi >> 2, base = (4 * hi) * 256 + (fi & 3) * 4 + (c >> 1) * 16;
         const int at[2] = {base + (c & 1) * 128, base + ((c & 1) ^ 1) * 128};
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb)
+        for (int rb = 0; rb < RBK; ++rb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int row_l = rb * 32 + (r & 3) + 8 * (r >> 2);
-                *(float*)(reg + row_l * 256 + at[r & 1]) = acc[2 * Q + rb][0][r];
-                *(float*)(reg + row_l * 256 + at[r & 1] + 64) = acc[2 * Q + rb][1][r];
+                *(float*)(reg + row_l * 256 + at[r & 1]) = acc[RBK * Q + rb][0][r];
+                *(float*)(reg + row_l * 256 + at[r & 1] + 64) = acc[RBK * Q + rb][1][r];
             }
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-            const int row_l = it * 8 + rl, row = m0 + Q * 64 + row_l;
+        for (int it = 0; it < IT; ++it) {
+            const int row_l = it * 8 + rl, row = m0 + Q * 32 * RBK + row_l;
             const f32x4_t lo = *(const f32x4_t*)(reg + row_l * 256 + q * 16 + (rl & 1) * 128), up = *(const f32x4_t*)(reg + row_l * 256 + q * 16 + ((rl & 1) ^ 1) * 128);
             float v[8] = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
 #pragma unroll
@@ -113,7 +117,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
                     if (RES == FW_DT_F32) { v[j] += __uint_as_float(rv[it][0][j]); v[4 + j] += __uint_as_float(rv[it][RES == FW_DT_F32 ? 1 : 0][j]); }
                     else { v[2 * j] += __uint_as_float(rv[it][0][j] << 16); v[2 * j + 1] += __uint_as_float(rv[it][0][j] & 0xffff0000u); }
                 }
-                if (Q + 1 < NQ) load_res(it, row + 64);
+                if (Q + 1 < NQ) load_res(it, row + 32 * RBK);
             } else if (res_dtype != FW_DT_NONE && live) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -163,92 +167,122 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
 
 // The combinations the engine runs are compiled on their own (each activation without a residual, either residual without an activation);
 // the others, and rows that cannot be accessed 16 bytes at a time, decide per element.
-template <int NQ, typename Acc>
+template <int RBK, int NQ, typename Acc>
 __device__ __forceinline__ void mx_finish(const MxArgs& p, char* reg, const Acc& acc, int lane, int m0, int n0) {
-    if (!p.vec) { mx_epilogue<-1, -1, false, NQ>(p, reg, acc, lane, m0, n0); return; }
+    if (!p.vec) { mx_epilogue<-1, -1, false, RBK, NQ>(p, reg, acc, lane, m0, n0); return; }
     if (p.res_dtype == FW_DT_NONE) {
         switch (p.act) {
-            case FW_ACT_RELU: mx_epilogue<FW_ACT_RELU, 0, true, NQ>(p, reg, acc, lane, m0, n0); break;
-            case FW_ACT_GELU_TANH: mx_epilogue<FW_ACT_GELU_TANH, 0, true, NQ>(p, reg, acc, lane, m0, n0); break;
-            case FW_ACT_GELU_ERF: mx_epilogue<FW_ACT_GELU_ERF, 0, true, NQ>(p, reg, acc, lane, m0, n0); break;
-            case FW_ACT_SILU: mx_epilogue<FW_ACT_SILU, 0, true, NQ>(p, reg, acc, lane, m0, n0); break;
-            default: mx_epilogue<FW_ACT_NONE, 0, true, NQ>(p, reg, acc, lane, m0, n0); break;
+            case FW_ACT_RELU: mx_epilogue<FW_ACT_RELU, 0, true, RBK, NQ>(p, reg, acc, lane, m0, n0); break;
+            case FW_ACT_GELU_TANH: mx_epilogue<FW_ACT_GELU_TANH, 0, true, RBK, NQ>(p, reg, acc, lane, m0, n0); break;
+            case FW_ACT_GELU_ERF: mx_epilogue<FW_ACT_GELU_ERF, 0, true, RBK, NQ>(p, reg, acc, lane, m0, n0); break;
+            case FW_ACT_SILU: mx_epilogue<FW_ACT_SILU, 0, true, RBK, NQ>(p, reg, acc, lane, m0, n0); break;
+            default: mx_epilogue<FW_ACT_NONE, 0, true, RBK, NQ>(p, reg, acc, lane, m0, n0); break;
         }
-    } else if (p.act != FW_ACT_NONE) mx_epilogue<-1, -1, true, NQ>(p, reg, acc, lane, m0, n0);
-    else if (p.res_dtype == FW_DT_F32) mx_epilogue<FW_ACT_NONE, FW_DT_F32, true, NQ>(p, reg, acc, lane, m0, n0);
-    else mx_epilogue<FW_ACT_NONE, FW_DT_BF16, true, NQ>(p, reg, acc, lane, m0, n0);
+    } else if (p.act != FW_ACT_NONE) mx_epilogue<-1, -1, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
+    else if (p.res_dtype == FW_DT_F32) mx_epilogue<FW_ACT_NONE, FW_DT_F32, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
+    else mx_epilogue<FW_ACT_NONE, FW_DT_BF16, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// 128 x 128 tile, 4 waves (2 x 2, wave tile 64 x 64), K slabs of 256 in two 32 KiB stages: two work-groups per CU.
+// BM x BN tiles, K slabs of 256 values in a ring of ST stages: four waves multiply (wave tile 32 x 64 at 64 x 128, 64 x 64 at 64 x 256, 128 x 64
+// at 128 x 256), four others do nothing but request codes and scale bytes by LDS-DMA, ST - 1 slabs ahead; one barrier a slab.  A slab past
+// the end is requested out of the descriptors' range (zeros into a stage that nobody reads any more), so the loaders' counted wait is the
+// same number in every iteration.
+// Why loaders of their own: a wave that requests its slab is held until the CU's path from L2 (64 bytes a clock) has taken the request, and
+// with one multiplying wave on a SIMD nobody multiplies meanwhile -- 257 x 5120 x 13824 took 39 us with four waves doing both, at two stages
+// as at four, and takes 21.7 with loaders.  What bounds it now is LDS (the waves' fragment reads and the DMA's writes: 574, 840 and 1150
+// clocks a slab of the three tiles, against 256, 512 and 1024 of the matrix pipe) and, per slab, the latency from the barrier to the first
+// fragments.  Time of a slab with one tile a CU: 0.37, 0.58 and 0.93 us.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int SM = 128, SN = 128, SSTAGE = (SM + SN) * 128;
-
-__global__ __launch_bounds__(256, 2) void gemm_mxfp4_128_kernel(MxArgs p) {
-    __shared__ __attribute__((aligned(16))) char smem[2 * SSTAGE];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave >> 1, wn = wave & 1, fi = lane & 31, hi = lane >> 5;
+template <int BM, int BN, int ST>
+__global__ __launch_bounds__(512, ST * (BM + BN) * 136 <= 80 * 1024 ? 4 : 2) void gemm_mxfp4_ring_kernel(MxArgs p) {
+    constexpr int WAVES_N = BN / 64, WAVES_M = 4 / WAVES_N;
+    constexpr int WM = BM / WAVES_M / 32;                 // 32-row blocks of a wave; it has two 32-column blocks
+    constexpr int APC = BM / 32, WPC = BN / 32;           // DMA pieces (8 rows x 128 bytes) of a wave and slab
+    constexpr int RB = (BM + BN) / 32;                    // 32-row groups of a slab = 256-byte scale tiles
+    constexpr int SPC = (RB + 3) / 4;                     // scale pieces of a wave (a wave past the last group repeats it)
+    constexpr int STAGE = (BM + BN) * 136;
+    constexpr int LDS = ST * STAGE > 4 * 16384 ? ST * STAGE : 4 * 16384;
+    __shared__ __attribute__((aligned(16))) char smem[LDS];
+    const int lane = threadIdx.x & 63, wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wave8 & 3;
+    const int wm = wave / WAVES_N, wn = wave % WAVES_N, fi = lane & 31, hi = lane >> 5;
     int tm, tn;
     mx_tile(p, tm, tn);
-    const int m0 = tm * SM, n0 = tn * SN;
-    const auto ars = mx_rsrc(p.A + (int64_t)m0 * p.lda, (long long)(p.M - m0) * p.lda);
-    const auto wrs = mx_rsrc(p.W + (int64_t)n0 * p.ldw, (long long)(p.N - n0) * p.ldw);
-    // a DMA piece = 8 rows x 128 bytes; this wave's pieces of a slab: rows 32 wave .. 32 wave + 31 of both operands
+    const int m0 = tm * BM, n0 = tn * BN;
+    // descriptors of this tile's rows alone: below 2^30 bytes, so PAST lies outside of every one
+    constexpr int PAST = 0x7f000000;
+    const auto ars = mx_rsrc(p.A + (int64_t)m0 * p.lda, (long long)min(p.M - m0, BM) * p.lda);
+    const auto wrs = mx_rsrc(p.W + (int64_t)n0 * p.ldw, (long long)min(p.N - n0, BN) * p.ldw);
+    const int sstride = __builtin_amdgcn_readfirstlane(p.slabs * 256);
+    const auto sars = mx_rsrc(p.sa + (int64_t)(m0 >> 5) * sstride, (long long)min((p.M + 31) / 32 - (m0 >> 5), BM / 32) * sstride);
+    const auto swrs = mx_rsrc(p.sw + (int64_t)(n0 >> 5) * sstride, (long long)min((p.N + 31) / 32 - (n0 >> 5), BN / 32) * sstride);
     const int pr = lane >> 3, pc = lane & 7;
     const int va[2] = {pr * (int)p.lda + ((pc ^ (pr >> 1)) << 4), pr * (int)p.lda + ((pc ^ ((pr >> 1) | 4)) << 4)};
     const int vw[2] = {pr * (int)p.ldw + ((pc ^ (pr >> 1)) << 4), pr * (int)p.ldw + ((pc ^ ((pr >> 1) | 4)) << 4)};
     const int astep = __builtin_amdgcn_readfirstlane((int)p.lda * 8), wstep = __builtin_amdgcn_readfirstlane((int)p.ldw * 8);
-    auto issue = [&](int st, int kt) __attribute__((always_inline)) {
+    auto issue = [&](char* st, int kt) __attribute__((always_inline)) {
+        const int k0 = kt < p.slabs ? kt * 128 : PAST, s0 = kt < p.slabs ? kt * 256 : PAST;
+        const int live = kt < p.slabs ? 1 : 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) FWX_BLDS16(ars, va[j & 1], kt * 128 + (wave * 4 + j) * astep, smem + st * SSTAGE + (wave * 4 + j) * 1024);
+        for (int j = 0; j < APC; ++j) FWX_BLDS16(ars, va[j & 1], k0 + live * (wave * APC + j) * astep, st + (wave * APC + j) * 1024);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) FWX_BLDS16(wrs, vw[j & 1], kt * 128 + (wave * 4 + j) * wstep, smem + st * SSTAGE + SM * 128 + (wave * 4 + j) * 1024);
+        for (int j = 0; j < WPC; ++j) FWX_BLDS16(wrs, vw[j & 1], k0 + live * (wave * WPC + j) * wstep, st + BM * 128 + (wave * WPC + j) * 1024);
+#pragma unroll
+        for (int j = 0; j < SPC; ++j) {
+            const int g = min(wave + 4 * j, RB - 1);
+            char* d = st + (BM + BN) * 128 + g * 256;
+            if (g < BM / 32) __builtin_amdgcn_raw_ptr_buffer_load_lds(sars, FW_LDS_PTR(d), 4, lane * 4, s0 + live * g * sstride, 0, 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(swrs, FW_LDS_PTR(d), 4, lane * 4, s0 + live * (g - BM / 32) * sstride, 0, 0);
+        }
     };
-    // scale dwords: one per 32 rows and slab; row blocks past the end repeat the last one (their rows are zeros and are never stored)
-    const int rba = (p.M + 31) / 32 - 1, rbw = (p.N + 31) / 32 - 1;
-    const uint8_t* sap[2];
-    const uint8_t* swp[2];
+    const int swz = (fi >> 1) & 7;
+    const int a_row = (wm * WM * 32 + fi) * 128, w_row = BM * 128 + (wn * 64 + fi) * 128;
+    const int s_a = (BM + BN) * 128 + wm * WM * 256 + fi * 8 + hi * 4, s_w = (BM + BN) * 128 + (BM / 32 + wn * 2) * 256 + fi * 8 + hi * 4;
+
+    if (wave8 >= 4) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        sap[i] = p.sa + (int64_t)min((m0 >> 5) + wm * 2 + i, rba) * p.slabs * 256 + fi * 8 + hi * 4;
-        swp[i] = p.sw + (int64_t)min((n0 >> 5) + wn * 2 + i, rbw) * p.slabs * 256 + fi * 8 + hi * 4;
+        for (int i = 0; i < ST - 1; ++i) issue(smem + i * STAGE, i);
+        int nxt = ST - 1;                                 // stage of slab kt + ST - 1: that of kt - 1
+        for (int kt = 0; kt < p.slabs; ++kt) {
+            mx_wait_vm<(ST - 2) * (APC + WPC + SPC)>();   // this wave's pieces of slab kt ...
+            FWX_BARRIER();                                // ... and every loader's; the others have read slab kt - 1
+            issue(smem + nxt * STAGE, kt + ST - 1);
+            nxt = nxt + 1 == ST ? 0 : nxt + 1;
+        }
+        mx_wait_vm<0>();                                  // the requests past the end
+        FWX_BARRIER();
+        return;
     }
-    int sca[2], scw[2];
-    auto scales = [&](int kt) __attribute__((always_inline)) {
+    f32x16_t acc[WM][2];                                  // [32-row block][32-column block]
 #pragma unroll
-        for (int i = 0; i < 2; ++i) { sca[i] = *(const int*)(sap[i] + (int64_t)kt * 256); scw[i] = *(const int*)(swp[i] + (int64_t)kt * 256); }
-    };
-    f32x16_t acc[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < WM; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-
-    const int swz = (fi >> 1) & 7;
-    scales(0);
-    issue(0, 0);
+    int cur = 0;
     for (int kt = 0; kt < p.slabs; ++kt) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's pieces of slab kt ...
-        __syncthreads();                                  // ... and everybody's; nobody reads the other stage any more
-        const char* a = smem + (kt & 1) * SSTAGE + (wm * 64 + fi) * 128;
-        const char* w = smem + (kt & 1) * SSTAGE + SM * 128 + (wn * 64 + fi) * 128;
-        const int ca[2] = {sca[0], sca[1]}, cw[2] = {scw[0], scw[1]};
-        if (kt + 1 < p.slabs) { scales(kt + 1); issue((kt + 1) & 1, kt + 1); }
+        FWX_BARRIER();
+        const char* st = smem + cur * STAGE;
+        int ca[WM], cw[2];
+#pragma unroll
+        for (int i = 0; i < WM; ++i) ca[i] = *(const int*)(st + s_a + i * 256);
+        cw[0] = *(const int*)(st + s_w);
+        cw[1] = *(const int*)(st + s_w + 256);
 #define FWX_STEP(J) do { \
             const int off = ((4 * hi + (J)) ^ swz) << 4; \
-            const i32x4_t a0 = *(const i32x4_t*)(a + off), a1 = *(const i32x4_t*)(a + 32 * 128 + off); \
-            const i32x4_t w0 = *(const i32x4_t*)(w + off), w1 = *(const i32x4_t*)(w + 32 * 128 + off); \
-            acc[0][0] = FWX_MFMA(a0, w0, acc[0][0], J, ca[0], cw[0]); \
-            acc[0][1] = FWX_MFMA(a0, w1, acc[0][1], J, ca[0], cw[1]); \
-            acc[1][0] = FWX_MFMA(a1, w0, acc[1][0], J, ca[1], cw[0]); \
-            acc[1][1] = FWX_MFMA(a1, w1, acc[1][1], J, ca[1], cw[1]); } while (0)
+            const i32x4_t w0 = *(const i32x4_t*)(st + w_row + off), w1 = *(const i32x4_t*)(st + w_row + 32 * 128 + off); \
+            _Pragma("unroll") for (int i = 0; i < WM; ++i) { \
+                const i32x4_t a0 = *(const i32x4_t*)(st + a_row + i * 32 * 128 + off); \
+                acc[i][0] = FWX_MFMA(a0, w0, acc[i][0], J, ca[i], cw[0]); \
+                acc[i][1] = FWX_MFMA(a0, w1, acc[i][1], J, ca[i], cw[1]); } } while (0)
         FWX_STEP(0); FWX_STEP(1); FWX_STEP(2); FWX_STEP(3);
 #undef FWX_STEP
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        cur = cur + 1 == ST ? 0 : cur + 1;
     }
-    __syncthreads();                                      // everybody has read the last slab: the stages become the epilogue's space
-    mx_finish<1>(p, smem + wave * 16384, acc, lane, m0 + wm * 64, n0 + wn * 64);
+    FWX_BARRIER();                                        // everybody has read the last slab: the stages become the epilogue's space
+    mx_finish<(WM < 2 ? 1 : 2), (WM < 2 ? 1 : WM / 2)>(p, smem + wave * 16384, acc, lane, m0 + wm * WM * 32, n0 + wn * 64);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -265,9 +299,6 @@ __global__ __launch_bounds__(256, 2) void gemm_mxfp4_128_kernel(MxArgs p) {
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int LM = 256, LN = 256;
 constexpr int L_A_STAGE = LM * 128, L_W_BASE = 2 * L_A_STAGE, L_W_STAGE = LN * 128, L_LDS = L_W_BASE + 3 * L_W_STAGE;
-
-#define FWX_BARRIER() do { __builtin_amdgcn_sched_barrier(0); asm volatile("s_barrier" ::: "memory"); __builtin_amdgcn_sched_barrier(0); } while (0)
-template <int N> __device__ __forceinline__ void mx_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 __global__ __launch_bounds__(512, 2) void gemm_mxfp4_256_kernel(MxArgs p) {
     __shared__ __attribute__((aligned(16))) char smem[L_LDS];
@@ -407,25 +438,25 @@ __global__ __launch_bounds__(512, 2) void gemm_mxfp4_256_kernel(MxArgs p) {
     };
     if (grp == 0) { mainloop(std::integral_constant<int, 0>{}); FWX_BARRIER(); }
     else mainloop(std::integral_constant<int, 1>{});
-    mx_finish<2>(p, smem + wave * 16384, acc, lane, m0 + grp * 128, n0 + wn * 64);
+    mx_finish<2, 2>(p, smem + wave * 16384, acc, lane, m0 + grp * 128, n0 + wn * 64);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Few rows (up to 64): the weights are all there is to read, so the split is made for them.  A work-group takes 16 NB columns (W rows) and all
+// Up to 16 rows: the weights are all there is to read, so the split is made for them.  A work-group takes 16 NB columns (W rows) and all
 // rows of A, its 8 waves a run of K each, v_mfma_scale_f32_16x16x128_f8f6f4 (lane l: row l & 15, block l >> 4 of four); a wave requests all
 // W of eight instructions before it multiplies, which keeps the whole matrix in flight across the chip.  The eight partial sums are added
 // in LDS, in wave order: no atomics, no workspace, the same bits every time.
-// FUSED (up to 16 rows): A is bf16 and the work-group quantises all of it into LDS, a block of 32 a lane, while its first W is on the way;
+// FUSED: A is bf16 and the work-group quantises all of it into LDS, a block of 32 a lane, while its first W is on the way;
 // every work-group repeats that, which costs less than a launch and a round trip through memory.  LDS rows are padded by one 16-byte chunk,
 // so the fragment reads of 16 rows hit 16 different chunks.
 // ---------------------------------------------------------------------------------------------------------------
 #define FWX_MFMA16(A, B, C, SA, SB) __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( \
     i32x8_t{(A)[0], (A)[1], (A)[2], (A)[3], 0, 0, 0, 0}, i32x8_t{(B)[0], (B)[1], (B)[2], (B)[3], 0, 0, 0, 0}, C, 4, 4, 0, SA, 0, SB)
 
-template <int MT, int NB, bool FUSED>
-__global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void gemm_mxfp4_rows_kernel(MxArgs p, int blocks) {
-    constexpr int UB = MT * NB == 1 ? 8 : 4;              // instructions (of 128 values of K) whose operands are requested together
-    __shared__ float red[8][MT * NB * 4][64];
+template <int NB, bool FUSED>
+__global__ __launch_bounds__(512, 4) void gemm_mxfp4_rows_kernel(MxArgs p, int blocks) {
+    constexpr int UB = NB == 1 ? 8 : 4;              // instructions (of 128 values of K) whose operands are requested together
+    __shared__ float red[8][NB * 4][64];
     extern __shared__ u32x4_t mx_rows[];                  // FUSED: codes [M][slabs * 8 + 1] chunks, then scale bytes [M][slabs * 8]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, h = lane >> 4;
@@ -440,23 +471,16 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void gemm_mxfp4_rows_kernel(M
         wp[b] = p.W + (int64_t)n * p.ldw + h * 16;
         swp[b] = p.sw + (int64_t)(n >> 5) * p.slabs * 256 + (n & 31) * 8 + h;
     }
-    const uint8_t* ap[MT];
-    const uint8_t* sap[MT];
     const int chunks = p.slabs * 8;                       // 16-byte chunks = blocks of a padded row
     uint8_t* smem_s = (uint8_t*)(mx_rows + p.M * (chunks + 1));
+    const int arow = min(r, p.M - 1);
+    const uint8_t* ap = FUSED ? (const uint8_t*)(mx_rows + arow * (chunks + 1) + h) : p.A + (int64_t)arow * p.lda + h * 16;
+    const uint8_t* sap = FUSED ? smem_s + arow * chunks + h : p.sa + arow * 8 + h;
+    f32x4_t acc[NB];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int row = min(m * 16 + r, p.M - 1);
-        ap[m] = FUSED ? (const uint8_t*)(mx_rows + row * (chunks + 1) + h) : p.A + (int64_t)row * p.lda + h * 16;
-        sap[m] = FUSED ? smem_s + row * chunks + h : p.sa + (int64_t)(row >> 5) * p.slabs * 256 + (row & 31) * 8 + h;
-    }
-    f32x4_t acc[MT][NB];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int b = 0; b < NB; ++b) acc[m][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    i32x4_t w[UB][NB], a[UB][MT];
-    int sw[UB][NB], sa[UB][MT];
+    for (int b = 0; b < NB; ++b) acc[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    i32x4_t w[UB][NB], a[UB];
+    int sw[UB][NB], sa[UB];
     auto load_w = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < UB; ++i)
@@ -492,36 +516,26 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void gemm_mxfp4_rows_kernel(M
 #pragma unroll
         for (int i = 0; i < UB; ++i)
             if (u + i < u1) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    a[i][m] = *(const i32x4_t*)(ap[m] + (int64_t)(u + i) * 64);
-                    sa[i][m] = FUSED ? sap[m][(u + i) * 4] : sap[m][(int64_t)((u + i) >> 1) * 256 + ((u + i) & 1) * 4];
-                }
+                a[i] = *(const i32x4_t*)(ap + (int64_t)(u + i) * 64);
+                sa[i] = FUSED ? sap[(u + i) * 4] : sap[(int64_t)((u + i) >> 1) * 256 + ((u + i) & 1) * 4];
             }
 #pragma unroll
         for (int i = 0; i < UB; ++i)
             if (u + i < u1) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) acc[m][b] = FWX_MFMA16(a[i][m], w[i][b], acc[m][b], sa[i][m], sw[i][b]);
+                for (int b = 0; b < NB; ++b) acc[b] = FWX_MFMA16(a[i], w[i][b], acc[b], sa[i], sw[i][b]);
             }
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) red[wave][(m * NB + b) * 4 + i][lane] = acc[m][b][i];
+        for (int i = 0; i < 4; ++i) red[wave][b * 4 + i][lane] = acc[b][i];
     __syncthreads();
     // lane l of a fragment holds column l & 15 of rows 4 (l >> 4) .. + 3
-    constexpr int COLS = 16 * NB, OUT = MT * 16 * COLS;
-#pragma unroll
-    for (int e0 = 0; e0 < OUT; e0 += 512) {
-        const int e = e0 + threadIdx.x;
-        if (OUT < 512 && e >= OUT) break;                 // whole waves: OUT is 256, or a multiple of 512
-        const int row = e / COLS, c = e % COLS, col = n0 + c;
-        const int slot = ((row >> 4) * NB + (c >> 4)) * 4 + (row & 3), at = ((row >> 2) & 3) * 16 + (c & 15);
+    constexpr int COLS = 16 * NB;
+    if (threadIdx.x < 16 * COLS) {                        // whole waves
+        const int row = threadIdx.x / COLS, c = threadIdx.x % COLS, col = n0 + c;
+        const int slot = (c >> 4) * 4 + (row & 3), at = (row >> 2) * 16 + (c & 15);
         float v = red[0][slot][at];
 #pragma unroll
         for (int k = 1; k < 8; ++k) v += red[k][slot][at];
@@ -553,11 +567,39 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void gemm_mxfp4_rows_kernel(M
     }
 }
 
-template <int MT, bool FUSED>
+template <int BM, int BN, int ST>
+int mx_launch_ring(MxArgs& p, int n_cover, hipStream_t st) {
+    p.tiles_m = (p.M + BM - 1) / BM; p.tiles_n = (n_cover + BN - 1) / BN;
+    const int64_t nwg = (int64_t)p.tiles_m * p.tiles_n;
+    if (nwg > 0x7fffffff) { fw_set_error("fw_gemm_mxfp4: grid too large"); return FW_E_BADARG; }
+    hipLaunchKernelGGL((gemm_mxfp4_ring_kernel<BM, BN, ST>), dim3((unsigned)nwg), dim3(512), 0, st, p);
+    return (int)hipGetLastError();
+}
+
+// Which tile: the one whose rounds over the 256 CUs, at its measured time of a slab and of the rest of a tile (ns), end first.
+//     tile        slab   rest      512 x 10240 x 5120   1565 x 5120 x 13824   2047 x 15360 x 5120   32760 x 15360 x 5120   (us)
+//     64 x 128     370   2000            24.0                 82.2                 116.6                 1873
+//     64 x 256     580   4000            28.6                 75.5                 119.6                 1830
+//     128 x 256    930   5000            22.3                103.5                  95.2                 1453
+//     256 x 256   1600  12000            31.5                102.7                  82.0                 1270
+// All of them add the same instructions in the same order per output element: a row's bits do not depend on the choice.
+int mx_tile_choice(int M, int n_cover, int slabs) {
+    static const int shape[4][4] = {{64, 128, 370, 2000}, {64, 256, 580, 4000}, {128, 256, 930, 5000}, {256, 256, 1600, 12000}};
+    int best = 0;
+    int64_t least = INT64_MAX;
+    for (int i = 0; i < (slabs >= 4 ? 4 : 3); ++i) {      // the 256 x 256 schedule needs four slabs
+        const int64_t tiles = (int64_t)((M + shape[i][0] - 1) / shape[i][0]) * ((n_cover + shape[i][1] - 1) / shape[i][1]);
+        const int64_t t = (tiles + 255) / 256 * ((int64_t)slabs * shape[i][2] + shape[i][3]);
+        if (t < least) { least = t; best = i; }
+    }
+    return best;
+}
+
+template <bool FUSED>
 int mx_launch_rows(const MxArgs& p, int n_cover, int blocks, hipStream_t st) {
     const int lds = FUSED ? p.M * (p.slabs * 8 + 1) * 16 + p.M * p.slabs * 8 : 0;
-    if (p.out_dtype == FW_DT_MXFP4) hipLaunchKernelGGL((gemm_mxfp4_rows_kernel<MT, 2, FUSED>), dim3((unsigned)((n_cover + 31) / 32)), dim3(512), lds, st, p, blocks);
-    else hipLaunchKernelGGL((gemm_mxfp4_rows_kernel<MT, 1, FUSED>), dim3((unsigned)((n_cover + 15) / 16)), dim3(512), lds, st, p, blocks);
+    if (p.out_dtype == FW_DT_MXFP4) hipLaunchKernelGGL((gemm_mxfp4_rows_kernel<2, FUSED>), dim3((unsigned)((n_cover + 31) / 32)), dim3(512), lds, st, p, blocks);
+    else hipLaunchKernelGGL((gemm_mxfp4_rows_kernel<1, FUSED>), dim3((unsigned)((n_cover + 15) / 16)), dim3(512), lds, st, p, blocks);
     return (int)hipGetLastError();
 }
 
@@ -607,14 +649,11 @@ extern "C" int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, c
     p.A = A; p.lda = lda; p.sa = sa;
     const int n_cover = out_dtype == FW_DT_MXFP4 ? cslabs * MX_SLAB : N;       // the padding of a quantised row is written too
     hipStream_t st = (hipStream_t)stream;
-    if (M <= 64) return M <= 16 ? mx_launch_rows<1, false>(p, n_cover, 0, st) : M <= 32 ? mx_launch_rows<2, false>(p, n_cover, 0, st) : mx_launch_rows<4, false>(p, n_cover, 0, st);
-    // 256 x 256 tiles from two full rounds' worth of rows and columns on; below, and for a tail of at most 128 rows past the last full
-    // tile (a whole extra round of 256-row tiles otherwise), the 128 x 128 kernel.  Both add the same instructions in the same order per
-    // output element: a row's bits do not depend on the kernel that computes it.
-    int m_big = 0;
-    if (M >= 2048 && N >= 1024 && slabs >= 4) {
-        const int tail = M % LM;
-        m_big = tail > 0 && tail <= SM ? M - tail : M;
+    if (M <= 16) return mx_launch_rows<false>(p, n_cover, 0, st);      // 16 x 5120 x 5120: 7.6 us, the 64 x 128 tiles 9.7; the same kernel for 32 rows took 10.4
+    int choice = mx_tile_choice(M, n_cover, slabs);
+    if (choice == 3) {
+        // a tail of at most 128 rows past the last full tile does not get a round of 256-row tiles: it goes by the same rule on its own
+        const int tail = M % LM, m_big = tail > 0 && tail <= 128 && M > LM ? M - tail : M;
         MxArgs b = p;
         b.M = m_big;
         b.tiles_m = (m_big + LM - 1) / LM; b.tiles_n = (n_cover + LN - 1) / LN;
@@ -623,17 +662,18 @@ extern "C" int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, c
         hipLaunchKernelGGL(gemm_mxfp4_256_kernel, dim3((unsigned)nwg), dim3(512), 0, st, b);
         const int rc = (int)hipGetLastError();
         if (rc || m_big == M) return rc;
+        // whole scale tiles (32 rows) lie behind, so the rest's scales and quantised output start on a tile of their own
+        p.A = A + (int64_t)m_big * lda; p.sa = sa + (int64_t)(m_big / 32) * slabs * 256; p.M = tail;
+        if (out_dtype == FW_DT_MXFP4) { p.C = (uint8_t*)C + (int64_t)m_big * ldc; p.cs = cs + (int64_t)(m_big / 32) * cslabs * 256; }
+        else p.C = (char*)C + (int64_t)m_big * ldc * (out_dtype == FW_DT_F32 ? 4 : 2);
+        if (res_dtype != FW_DT_NONE) p.res = (const char*)res + (int64_t)m_big * ldr * (res_dtype == FW_DT_F32 ? 4 : 2);
+        choice = min(mx_tile_choice(tail, n_cover, slabs), 2);
     }
-    // the rest: a multiple of 32 rows in, so scale tiles and quantised output start on a tile of their own
-    p.A = A + (int64_t)m_big * lda; p.sa = sa + (int64_t)(m_big / 32) * slabs * 256; p.M = M - m_big;
-    if (out_dtype == FW_DT_MXFP4) { p.C = (uint8_t*)C + (int64_t)m_big * ldc; p.cs = cs + (int64_t)(m_big / 32) * cslabs * 256; }
-    else p.C = (char*)C + (int64_t)m_big * ldc * (out_dtype == FW_DT_F32 ? 4 : 2);
-    if (res_dtype != FW_DT_NONE) p.res = (const char*)res + (int64_t)m_big * ldr * (res_dtype == FW_DT_F32 ? 4 : 2);
-    p.tiles_m = (p.M + SM - 1) / SM; p.tiles_n = (n_cover + SN - 1) / SN;
-    const int64_t nwg = (int64_t)p.tiles_m * p.tiles_n;
-    if (nwg > 0x7fffffff) { fw_set_error("fw_gemm_mxfp4: grid too large"); return FW_E_BADARG; }
-    hipLaunchKernelGGL(gemm_mxfp4_128_kernel, dim3((unsigned)nwg), dim3(256), 0, st, p);
-    return (int)hipGetLastError();
+    switch (choice) {
+        case 0: return mx_launch_ring<64, 128, 3>(p, n_cover, st);
+        case 1: return mx_launch_ring<64, 256, 3>(p, n_cover, st);
+        default: return mx_launch_ring<128, 256, 3>(p, n_cover, st);
+    }
 }
 
 extern "C" int64_t fw_linear_mxfp4_workspace_bytes(int M, int K) {
@@ -652,7 +692,7 @@ extern "C" int fw_linear_mxfp4(const uint16_t* x, int64_t ldx, const uint8_t* W,
         MxArgs p;
         if (const int rc = mx_args(p, W, ldw, sw, C, ldc, out_dtype, cs, M, N, K, bias, act, g1, g0, res, ldr, res_dtype)) return rc;
         p.A = (const uint8_t*)x; p.lda = ldx * 2; p.sa = nullptr;
-        return mx_launch_rows<1, true>(p, out_dtype == FW_DT_MXFP4 ? p.cslabs * MX_SLAB : N, K / 32, (hipStream_t)stream);
+        return mx_launch_rows<true>(p, out_dtype == FW_DT_MXFP4 ? p.cslabs * MX_SLAB : N, K / 32, (hipStream_t)stream);
     }
     if (!workspace || workspace_bytes < fw_linear_mxfp4_workspace_bytes(M, K) || (((uintptr_t)workspace) & 15)) {
         fw_set_error("fw_linear_mxfp4: a 16-byte aligned workspace of fw_linear_mxfp4_workspace_bytes(M, K) required"); return FW_E_BADARG; }
