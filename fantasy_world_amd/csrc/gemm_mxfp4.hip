@@ -51,61 +51,95 @@ __device__ __forceinline__ void mx_tile(const MxArgs& p, int& tm, int& tn) {
     tn = in_g / gsz;
 }
 
-// Epilogue of NQ quadrants (32 RBK x 64 each, stacked along M) of a wave: accumulators -> LDS (16 KiB of the wave's own) -> rows -> bias,
-// activation, per-column affine, residual, store.  A lane owns 8 consecutive columns of a row, 8 rows per step: 16-byte accesses in bf16,
-// and with MXFP4 output a block of 32 columns is the 4 lanes of a quad.
+// GELU with erf by Abramowitz & Stegun 7.1.26 (|error of erf| <= 1.5e-7), in its complementary form: no cancellation for negative values.
+// erff in its place costs 14 us per 128 x 256 tile.
+__device__ __forceinline__ float mx_gelu_erf(float x) {
+    const float z = fabsf(x) * 0.7071067811865476f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
+    float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    q = __builtin_fmaf(q, t, 1.421413741f);
+    q = __builtin_fmaf(q, t, -0.284496736f);
+    q = __builtin_fmaf(q, t, 0.254829592f);
+    return fmaxf(x, 0.f) - 0.5f * fabsf(x) * (q * t * __expf(-z * z));
+}
+template <int ACT>
+__device__ __forceinline__ float mx_act(float v) { return ACT == FW_ACT_GELU_ERF ? mx_gelu_erf(v) : fw_apply_act(v, ACT); }
+
+template <typename F>
+__device__ __forceinline__ void mx_by_act(int act, F&& f) {
+    switch (act) {
+        case FW_ACT_RELU: f(std::integral_constant<int, FW_ACT_RELU>{}); break;
+        case FW_ACT_GELU_TANH: f(std::integral_constant<int, FW_ACT_GELU_TANH>{}); break;
+        case FW_ACT_GELU_ERF: f(std::integral_constant<int, FW_ACT_GELU_ERF>{}); break;
+        case FW_ACT_SILU: f(std::integral_constant<int, FW_ACT_SILU>{}); break;
+        default: f(std::integral_constant<int, FW_ACT_NONE>{}); break;
+    }
+}
+
+// Epilogue of NQ quadrants (32 RBK x 64 each, stacked along M) of a wave: bias and activation on the accumulators (a lane holds one column
+// of each 32 x 32 block), then through LDS (16 KiB of the wave's own) to rows, per-column affine, residual, store.  There a lane owns 8
+// consecutive columns of a row, 8 rows per step: 16-byte accesses in bf16, and with MXFP4 output a block of 32 columns is the 4 lanes of a
+// quad.
 // LDS image: 16-byte chunk c of row r lies at (c >> 1) + 8 ((c ^ r) & 1) of the row's 16: the 16 lanes of a read (chunk 2q or 2q + 1 of two
 // neighbouring rows) then hit 16 different chunks of the 64 banks.
-// ACT, RES < 0: decided per element at run time.  VEC: every row of C and of the residual is 16-byte accessible and N % 8 == 0.
-// With a residual the 64 rows' loads are all in flight before the transpose, and the next quadrant's are issued as registers free up:
-// read one step at a time they cost a memory latency each (32 us per 256 x 256 tile with an fp32 residual, against 32 us of main loop).
-template <int ACT, int RES, bool VEC, int RBK, int NQ, typename Acc>
+// VEC: every row of C and of the residual is 16-byte accessible and N % 8 == 0; otherwise (and RES < 0) element by element.
+// With a residual and no activation all of a quadrant's residual rows are in flight before the transpose and the next quadrant's are issued
+// as registers free up; with an activation as well (ACT_TOO) they follow the transpose, in the registers that the accumulators leave.
+template <int RES, bool VEC, bool ACT_TOO, int RBK, int NQ, typename Acc>
 __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Acc& acc, int lane, int m0, int n0) {
     const int fi = lane & 31, hi = lane >> 5, q = lane & 7, rl = lane >> 3;
     const int col = n0 + q * 8;
     const bool in = col < p.N;
     const int res_dtype = RES < 0 ? p.res_dtype : RES;
-    float bias[8], g1[8], g0[8];
-    const bool affine = p.g1 || p.g0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        bias[j] = p.bias && col + j < p.N ? p.bias[col + j] : 0.f;
-        g1[j] = p.g1 && col + j < p.N ? p.g1[col + j] : 1.f;
-        g0[j] = p.g0 && col + j < p.N ? p.g0[col + j] : 0.f;
-    }
     constexpr int IT = 4 * RBK;                           // steps of 8 rows
     u32x4_t rv[IT][RES == FW_DT_F32 ? 2 : 1];
-    auto load_res = [&](int it, int row) __attribute__((always_inline)) {
+    auto load_res = [&](int it, int row0) __attribute__((always_inline)) {
+        const int row = row0 + rl;
         if (VEC && RES > 0 && in && row < p.M) {
-            const char* r = (const char*)p.res + ((int64_t)row * p.ldr + col) * (RES == FW_DT_F32 ? 4 : 2);
+            // a scalar row address and a 32-bit lane offset: 64-bit addresses of 16 loads do not fit next to the accumulators
+            const char* r = (const char*)p.res + ((int64_t)row0 * p.ldr + n0) * (RES == FW_DT_F32 ? 4 : 2) + (unsigned)(rl * (int)p.ldr + q * 8) * (RES == FW_DT_F32 ? 4u : 2u);
             rv[it][0] = *(const u32x4_t*)r;
             if (RES == FW_DT_F32) rv[it][RES == FW_DT_F32 ? 1 : 0] = *(const u32x4_t*)(r + 16);
         }
     };
-    if (VEC && RES > 0) {
+    if (VEC && RES > 0 && !ACT_TOO) {
 #pragma unroll
-        for (int it = 0; it < IT; ++it) load_res(it, m0 + it * 8 + rl);
+        for (int it = 0; it < IT; ++it) load_res(it, m0 + it * 8);
+    }
+    float g1[8], g0[8], bias[2];
+    const bool affine = p.g1 || p.g0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) bias[j] = p.bias && n0 + j * 32 + fi < p.N ? p.bias[n0 + j * 32 + fi] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        g1[j] = p.g1 && col + j < p.N ? p.g1[col + j] : 1.f;
+        g0[j] = p.g0 && col + j < p.N ? p.g0[col + j] : 0.f;
     }
     auto quadrant = [&](auto q_tag) __attribute__((always_inline)) {
         constexpr int Q = decltype(q_tag)::value;
         // chunk of column fi: fi >> 2, of column 32 + fi: 8 + (fi >> 2); rows of a register pair alternate in parity
         const int c = fi >> 2, base = (4 * hi) * 256 + (fi & 3) * 4 + (c >> 1) * 16;
         const int at[2] = {base + (c & 1) * 128, base + ((c & 1) ^ 1) * 128};
+        mx_by_act(ACT_TOO ? p.act : FW_ACT_NONE, [&](auto act_tag) __attribute__((always_inline)) {
+            constexpr int ACT = decltype(act_tag)::value;
 #pragma unroll
-        for (int rb = 0; rb < RBK; ++rb)
+            for (int rb = 0; rb < RBK; ++rb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row_l = rb * 32 + (r & 3) + 8 * (r >> 2);
-                *(float*)(reg + row_l * 256 + at[r & 1]) = acc[RBK * Q + rb][0][r];
-                *(float*)(reg + row_l * 256 + at[r & 1] + 64) = acc[RBK * Q + rb][1][r];
-            }
+                for (int r = 0; r < 16; ++r) {
+                    const int row_l = rb * 32 + (r & 3) + 8 * (r >> 2);
+                    *(float*)(reg + row_l * 256 + at[r & 1]) = mx_act<ACT>(acc[RBK * Q + rb][0][r] + bias[0]);
+                    *(float*)(reg + row_l * 256 + at[r & 1] + 64) = mx_act<ACT>(acc[RBK * Q + rb][1][r] + bias[1]);
+                }
+        });
+        if (VEC && RES > 0 && ACT_TOO) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int it = 0; it < IT; ++it) load_res(it, m0 + Q * 32 * RBK + it * 8);
+        }
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
             const int row_l = it * 8 + rl, row = m0 + Q * 32 * RBK + row_l;
             const f32x4_t lo = *(const f32x4_t*)(reg + row_l * 256 + q * 16 + (rl & 1) * 128), up = *(const f32x4_t*)(reg + row_l * 256 + q * 16 + ((rl & 1) ^ 1) * 128);
             float v[8] = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = fw_apply_act(v[j] + bias[j], ACT < 0 ? p.act : ACT);
             if (affine) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = fw_affine(v[j], g1[j], g0[j]);
@@ -117,7 +151,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
                     if (RES == FW_DT_F32) { v[j] += __uint_as_float(rv[it][0][j]); v[4 + j] += __uint_as_float(rv[it][RES == FW_DT_F32 ? 1 : 0][j]); }
                     else { v[2 * j] += __uint_as_float(rv[it][0][j] << 16); v[2 * j + 1] += __uint_as_float(rv[it][0][j] & 0xffff0000u); }
                 }
-                if (Q + 1 < NQ) load_res(it, row + 32 * RBK);
+                if (Q + 1 < NQ && !ACT_TOO) load_res(it, m0 + (Q + 1) * 32 * RBK + it * 8);
             } else if (res_dtype != FW_DT_NONE && live) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -165,22 +199,16 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
     if constexpr (NQ > 1) quadrant(std::integral_constant<int, 1>{});
 }
 
-// The combinations the engine runs are compiled on their own (each activation without a residual, either residual without an activation);
-// the others, and rows that cannot be accessed 16 bytes at a time, decide per element.
 template <int RBK, int NQ, typename Acc>
 __device__ __forceinline__ void mx_finish(const MxArgs& p, char* reg, const Acc& acc, int lane, int m0, int n0) {
-    if (!p.vec) { mx_epilogue<-1, -1, false, RBK, NQ>(p, reg, acc, lane, m0, n0); return; }
-    if (p.res_dtype == FW_DT_NONE) {
-        switch (p.act) {
-            case FW_ACT_RELU: mx_epilogue<FW_ACT_RELU, 0, true, RBK, NQ>(p, reg, acc, lane, m0, n0); break;
-            case FW_ACT_GELU_TANH: mx_epilogue<FW_ACT_GELU_TANH, 0, true, RBK, NQ>(p, reg, acc, lane, m0, n0); break;
-            case FW_ACT_GELU_ERF: mx_epilogue<FW_ACT_GELU_ERF, 0, true, RBK, NQ>(p, reg, acc, lane, m0, n0); break;
-            case FW_ACT_SILU: mx_epilogue<FW_ACT_SILU, 0, true, RBK, NQ>(p, reg, acc, lane, m0, n0); break;
-            default: mx_epilogue<FW_ACT_NONE, 0, true, RBK, NQ>(p, reg, acc, lane, m0, n0); break;
-        }
-    } else if (p.act != FW_ACT_NONE) mx_epilogue<-1, -1, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
-    else if (p.res_dtype == FW_DT_F32) mx_epilogue<FW_ACT_NONE, FW_DT_F32, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
-    else mx_epilogue<FW_ACT_NONE, FW_DT_BF16, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
+    const bool act = p.act != FW_ACT_NONE;
+    if (!p.vec) mx_epilogue<-1, false, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
+    else if (p.res_dtype == FW_DT_NONE) mx_epilogue<FW_DT_NONE, true, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
+    else if (p.res_dtype == FW_DT_F32) {
+        if (act) mx_epilogue<FW_DT_F32, true, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
+        else mx_epilogue<FW_DT_F32, true, false, RBK, NQ>(p, reg, acc, lane, m0, n0);
+    } else if (act) mx_epilogue<FW_DT_BF16, true, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
+    else mx_epilogue<FW_DT_BF16, true, false, RBK, NQ>(p, reg, acc, lane, m0, n0);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -541,7 +569,7 @@ __global__ __launch_bounds__(512, 4) void gemm_mxfp4_rows_kernel(MxArgs p, int b
         for (int k = 1; k < 8; ++k) v += red[k][slot][at];
         const bool in = col < p.N, live = row < p.M;
         if (p.bias && in) v += p.bias[col];
-        v = fw_apply_act(v, p.act);
+        mx_by_act(p.act, [&](auto act) __attribute__((always_inline)) { v = mx_act<decltype(act)::value>(v); });
         if ((p.g1 || p.g0) && in) v = fw_affine(v, p.g1 ? p.g1[col] : 1.f, p.g0 ? p.g0[col] : 0.f);
         if (p.res_dtype != FW_DT_NONE && in && live) {
             const int64_t o = (int64_t)row * p.ldr + col;
@@ -576,20 +604,23 @@ int mx_launch_ring(MxArgs& p, int n_cover, hipStream_t st) {
     return (int)hipGetLastError();
 }
 
-// Which tile: the one whose rounds over the 256 CUs, at its measured time of a slab and of the rest of a tile (ns), end first.
-//     tile        slab   rest      512 x 10240 x 5120   1565 x 5120 x 13824   2047 x 15360 x 5120   32760 x 15360 x 5120   (us)
-//     64 x 128     370   2000            24.0                 82.2                 116.6                 1873
-//     64 x 256     580   4000            28.6                 75.5                 119.6                 1830
-//     128 x 256    930   5000            22.3                103.5                  95.2                 1453
-//     256 x 256   1600  12000            31.5                102.7                  82.0                 1270
+// Which tile: the one whose rounds over the 256 CUs, at its measured time of a slab and of the rest of a tile (ns), end first.  A slab takes
+// half as long on a nearly empty chip as on a full one (clock, L2); 64 x 128 tiles run two to a CU from 257 of them on.
+//     tile        slab   rest      512 x 10240 x 5120   1565 x 5120 x 13824   2047 x 15360 x 5120   32760 x 15360 x 5120   (us measured)
+//     64 x 128     300   2500            24.0                 82.2                 116.6                 1873
+//     64 x 256     560   5000            28.6                 75.5                 119.6                 1830
+//     128 x 256    950   7500            22.3                103.5                  95.2                 1453
+//     256 x 256   1550  11000            31.5                102.7                  82.0                 1270
 // All of them add the same instructions in the same order per output element: a row's bits do not depend on the choice.
 int mx_tile_choice(int M, int n_cover, int slabs) {
-    static const int shape[4][4] = {{64, 128, 370, 2000}, {64, 256, 580, 4000}, {128, 256, 930, 5000}, {256, 256, 1600, 12000}};
+    static const int shape[4][4] = {{64, 128, 300, 2500}, {64, 256, 560, 5000}, {128, 256, 950, 7500}, {256, 256, 1550, 11000}};
     int best = 0;
     int64_t least = INT64_MAX;
     for (int i = 0; i < (slabs >= 4 ? 4 : 3); ++i) {      // the 256 x 256 schedule needs four slabs
         const int64_t tiles = (int64_t)((M + shape[i][0] - 1) / shape[i][0]) * ((n_cover + shape[i][1] - 1) / shape[i][1]);
-        const int64_t t = (tiles + 255) / 256 * ((int64_t)slabs * shape[i][2] + shape[i][3]);
+        const int64_t rounds = (tiles + 255) / 256;
+        const int64_t slab = i > 0 ? shape[i][2] * (rounds * 256 + tiles) / (rounds * 512) : tiles > 256 ? 300 : 370;
+        const int64_t t = rounds * (slabs * slab + shape[i][3]);
         if (t < least) { least = t; best = i; }
     }
     return best;
@@ -632,7 +663,7 @@ static int mx_args(MxArgs& p, const uint8_t* W, int64_t ldw, const uint8_t* sw, 
     // 16-byte accesses of 8 columns in the epilogue
     const int ce = out_dtype == FW_DT_F32 ? 4 : 8, re = res_dtype == FW_DT_F32 ? 4 : 8;
     p.vec = (N % 8) == 0 && (out_dtype == FW_DT_MXFP4 || ((ldc % ce) == 0 && (((uintptr_t)C) & 15) == 0)) &&
-            (res_dtype == FW_DT_NONE || ((ldr % re) == 0 && (((uintptr_t)res) & 15) == 0));
+            (res_dtype == FW_DT_NONE || ((ldr % re) == 0 && (((uintptr_t)res) & 15) == 0 && ldr < (1 << 26)));
     return 0;
 }
 
