@@ -38,6 +38,9 @@ def _ru64(n):
     return (n + 63) // 64 * 64
 
 
+PRECISIONS = ("bf16", "fp8", "mxfp4")
+
+
 class _DitBlock:
     pass
 
@@ -103,13 +106,17 @@ class FusionEngine:
         geometry heads: joint_forward(return_prediction=True) then returns the reference's prediction dict
         (vggt.py:134-154); their weights are packed on first use.  `cache_step_invariants` keeps the intermediates that
         only depend on the prompt / camera inputs across calls (same results, bit for bit; see _InvariantCache).
-        `precision="fp8"` routes the DiT blocks' linears through the reference's fp8 linear; `fp8_attention=True` additionally
+        `precision="fp8"` routes the DiT blocks' linears through the reference's fp8 linear; `precision="mxfp4"` holds the same linears'
+        weights AND inputs as MXFP4 (include/fw_mi355x.h; no reference semantics): the norms in front of them write MXFP4 rows
+        (residual_norm), the first FFN linear hands its hidden rows to the second in MXFP4.  `fp8_attention=True` additionally
         runs the DiT self-attention (hd 128, 41 % of a step's FLOPs) on e4m3 q / k / v / probabilities (parity
         UNPINNED -- the reference defines no fp8 attention).  Under a sequence shard the head exchange then carries q | k | v as
         e4m3 BYTES (half the all-to-all payload) and every rank runs fw_attention_fp8 on the heads it received: the same bytes
         reach the same kernel, so the sharded forward returns the unsharded one's bits."""
-        if precision not in ("bf16", "fp8"):
-            raise ValueError(f"precision must be 'bf16' or 'fp8', got {precision!r}")
+        if precision not in PRECISIONS:
+            raise ValueError(f"precision must be one of {PRECISIONS}, got {precision!r}")
+        if precision == "mxfp4" and not hasattr(ops, "pack_linear_mxfp4"):
+            raise ValueError("precision 'mxfp4' needs an op set with the MXFP4 linear (fw_gemm_mxfp4)")
         if fp8_attention not in (False, True, "bicross", "all"):
             raise ValueError("fp8_attention: False | True (DiT self-attention) | 'bicross' (+ the bicross attention) | 'all' (+ the VGGT "
                              "frame / global attention on the head_dim-64 kernel); the last two are round-6 experiments, unsharded engine only")
@@ -202,11 +209,12 @@ class FusionEngine:
 
     # ------------------------------------------------------------------------------------------------ packing
     def _packers(self, get):
-        """(g, lin, lin_cat): fetch a reference parameter as fp32 / pack one nn.Linear / pack several as one fused projection."""
+        """(g, lin, lin_cat): fetch a reference parameter as fp32 / pack one nn.Linear / pack several as one fused projection
+        (fp8=True / mxfp4=True: for that linear instead of the bf16 one)."""
         ops_ = self.ops
         g = lambda n: get(n).detach().to(torch.float32)
 
-        def lin(wname, bname=None, k_pad=None, n_pad=None, fp8=False):
+        def lin(wname, bname=None, k_pad=None, n_pad=None, **kind):
             w = g(wname)
             w = w.reshape(w.shape[0], -1)
             b = g(bname) if bname else None
@@ -216,12 +224,12 @@ class FusionEngine:
                 w = _pad_to(w, 0, n_pad)
                 if b is not None:
                     b = _pad_to(b, 0, n_pad)
-            return ops_.pack_linear(w, b, fp8=True) if fp8 else ops_.pack_linear(w, b)
+            return ops_.pack_linear(w, b, **kind)
 
-        def lin_cat(names, fp8=False):
+        def lin_cat(names, **kind):
             w = torch.cat([g(n + ".weight") for n in names], dim=0)
             b = torch.cat([g(n + ".bias") for n in names], dim=0)
-            return ops_.pack_linear(w, b, fp8=True) if fp8 else ops_.pack_linear(w, b)
+            return ops_.pack_linear(w, b, **kind)
 
         return g, lin, lin_cat
 
@@ -235,19 +243,19 @@ class FusionEngine:
         # precision "fp8": the DiT block's nn.Linear modules are the ones enable_vram_management swaps for AutoWrappedLinear
         # (diffsynth_wan21/vram_management/layers.py:145-166, module_map {nn.Linear: AutoWrappedLinear}) -- q/k/v/o of both
         # attentions and the FFN go through the fp8 linear; norms, modulation, the camera adapter and everything outside the
-        # DiT blocks (embeddings, head, VGGT, bicross) keep the bf16 path
-        f8 = self.precision == "fp8"
-        blk.qkv = lin_cat([p + "self_attn.q", p + "self_attn.k", p + "self_attn.v"], fp8=f8)
-        blk.o = lin(p + "self_attn.o.weight", p + "self_attn.o.bias", fp8=f8)
+        # DiT blocks (embeddings, head, VGGT, bicross) keep the bf16 path.  precision "mxfp4": the same linears
+        kind = self._linear_kind()
+        blk.qkv = lin_cat([p + "self_attn.q", p + "self_attn.k", p + "self_attn.v"], **kind)
+        blk.o = lin(p + "self_attn.o.weight", p + "self_attn.o.bias", **kind)
         blk.norm_q = ops.to_f32(g(p + "self_attn.norm_q.weight"))
         blk.norm_k = ops.to_f32(g(p + "self_attn.norm_k.weight"))
-        blk.cq = lin(p + "cross_attn.q.weight", p + "cross_attn.q.bias", fp8=f8)
-        blk.ckv = lin_cat([p + "cross_attn.k", p + "cross_attn.v"], fp8=f8)
-        blk.co = lin(p + "cross_attn.o.weight", p + "cross_attn.o.bias", fp8=f8)
+        blk.cq = lin(p + "cross_attn.q.weight", p + "cross_attn.q.bias", **kind)
+        blk.ckv = lin_cat([p + "cross_attn.k", p + "cross_attn.v"], **kind)
+        blk.co = lin(p + "cross_attn.o.weight", p + "cross_attn.o.bias", **kind)
         blk.cnorm_q = ops.to_f32(g(p + "cross_attn.norm_q.weight"))
         blk.cnorm_k = ops.to_f32(g(p + "cross_attn.norm_k.weight"))
         if cfg.has_image_input:
-            blk.ckv_img = lin_cat([p + "cross_attn.k_img", p + "cross_attn.v_img"], fp8=f8)
+            blk.ckv_img = lin_cat([p + "cross_attn.k_img", p + "cross_attn.v_img"], **kind)
             blk.cnorm_k_img = ops.to_f32(g(p + "cross_attn.norm_k_img.weight"))
         blk.adapter = cfg.has_adapter(b) if adapter is None else bool(adapter)
         if blk.adapter:
@@ -260,9 +268,20 @@ class FusionEngine:
             blk.a_v2 = lin(a + "v_proj.group2.2.weight", a + "v_proj.group2.2.bias", k_pad=rp)   # 409 -> 448 cols (zeros)
         blk.norm3_w = ops.to_f32(g(p + "norm3.weight"))
         blk.norm3_b = ops.to_f32(g(p + "norm3.bias"))
-        blk.ffn0 = lin(p + "ffn.0.weight", p + "ffn.0.bias", fp8=f8)
-        blk.ffn2 = lin(p + "ffn.2.weight", p + "ffn.2.bias", fp8=f8)
+        blk.ffn0 = lin(p + "ffn.0.weight", p + "ffn.0.bias", **kind)
+        blk.ffn2 = lin(p + "ffn.2.weight", p + "ffn.2.bias", **kind)
         return blk
+
+    def _linear_kind(self):
+        """pack_linear's keywords for a DiT block's linears at this engine's precision."""
+        return {} if self.precision == "bf16" else {self.precision: True}
+
+    def _norm_into(self, lin, x, **kw):
+        """LayerNorm (+ affine, + modulation) of the stream as the input of `lin`: bf16 rows, or the MXFP4 rows an MXFP4 linear takes (one
+        pass: fw_residual_norm without an update; the codes of quantising the bf16 rows)."""
+        if getattr(lin, "mxfp4", False):
+            return self.ops.residual_norm(x, None, out="mxfp4", **kw)
+        return self.ops.layernorm(x, **kw)
 
     def _pack_vggt(self, p, g, lin):
         cfg, ops = self.cfg, self.ops
@@ -332,7 +351,7 @@ class FusionEngine:
         st = _Stage()
         st.blk, st.x, st.qkv8 = blk, x, None
         st.mod = self._dit_mod(blk, t_mod)                       # [6, D]: shift/scale/gate msa, shift/scale/gate mlp
-        xn = ops.layernorm(x, scale=st.mod[1], shift=st.mod[0], eps=cfg.eps)
+        xn = self._norm_into(blk.qkv, x, scale=st.mod[1], shift=st.mod[0], eps=cfg.eps)
         qkv = ops.linear(xn, blk.qkv)
         q, k = qkv[:, :D], qkv[:, D:2 * D]
         tab = tabs["dit"] if sh is None else tabs["dit_local"]
@@ -445,7 +464,7 @@ class FusionEngine:
             o = st.pend.wait()
         ops.linear(o, blk.o, g1=mod[2], res=x, out_f32=True, out=x)
         # cross-attention: text + image keys share q; outputs are summed (wan_video_dit.py:185-201)
-        xn3 = ops.layernorm(x, w=blk.norm3_w, b=blk.norm3_b, eps=cfg.eps)
+        xn3 = self._norm_into(blk.cq, x, w=blk.norm3_w, b=blk.norm3_b, eps=cfg.eps)
         qc = ops.linear(xn3, blk.cq)
         ops.qk_prep(qc, H, hd, norm="rms_full", norm_w=blk.cnorm_q, eps=cfg.eps, out_scale=ops.q_scale(hd))
         def text_kv():
@@ -505,8 +524,9 @@ class FusionEngine:
     def _dit_ffn(self, blk, x, mod):
         """FFN half (`run_remaining`, wan_video_dit.py:288-294)."""
         cfg, ops = self.cfg, self.ops
-        xn = ops.layernorm(x, scale=mod[4], shift=mod[3], eps=cfg.eps)
-        hbuf = ops.linear(xn, blk.ffn0, act="gelu_tanh")
+        xn = self._norm_into(blk.ffn0, x, scale=mod[4], shift=mod[3], eps=cfg.eps)
+        hidden = {"out_mxfp4": True} if getattr(blk.ffn2, "mxfp4", False) else {}
+        hbuf = ops.linear(xn, blk.ffn0, act="gelu_tanh", **hidden)
         ops.linear(hbuf, blk.ffn2, g1=mod[5], res=x, out_f32=True, out=x)
 
     def _vggt_attn_begin(self, blk, tok, e0, tabs, batch, frame_mode):

@@ -865,9 +865,9 @@ class HipOps:
 
     # ---- the seam between two halves of a block --------------------------------------------------------------------------------------
     def residual_norm(self, x, y=None, bias=None, g1=None, g0=None, post=None, post_w=None, w=None, b=None, scale=None, shift=None,
-                      norm="layer", eps=1e-6, x_out=None, out="bf16"):
+                      norm="layer", eps=1e-6, x_out=None, out="bf16", h_out=None):
         """x' = x + [post norm](y + bias) * g1 + g0, written to x_out (default: x, in place); -> h = norm(x') * w + b, * (1 + scale) + shift, as
-        bf16 rows or (out="mxfp4") MXFP4Rows.  y None: h alone.  x, x_out [rows, C] fp32 or bf16, y fp32 or bf16; bias / post_w / w / b [C];
+        bf16 rows (h_out: written there, rows may be strided) or (out="mxfp4") MXFP4Rows.  y None: h alone.  x, x_out [rows, C] fp32 or bf16, y fp32 or bf16; bias / post_w / w / b [C];
         g1 / g0 / scale / shift [C], or all of them [groups, C] with rows % groups == 0: equal runs of rows share a vector.  post: None, "layer" or "rms"
         (post_w only with it); norm: "layer" or "rms" (b only with w)."""
         ldx = self._rows("x", x, torch.float32, torch.bfloat16)
@@ -904,13 +904,21 @@ class HipOps:
                     raise ValueError(f"{name}: {n} vectors for {rows} rows; g1, g0, scale and shift alike in number, a divisor of the rows, expected")
                 groups = n
             ptrs.append(v.data_ptr())
-        st = self._enter(x, y, x_out, bias, g1, g0, post_w, w, b, scale, shift)
-        mx = MXFP4Rows._unwritten(rows, C, x.device) if out == "mxfp4" else None
-        if mx is None:
-            h = torch.empty((rows, C), dtype=torch.bfloat16, device=x.device)
-            hp, ldh, hdt, hsp = h.data_ptr(), C, FW_DT_BF16, 0
+        st = self._enter(x, y, x_out, bias, g1, g0, post_w, w, b, scale, shift, h_out)
+        if out == "mxfp4":
+            if h_out is not None:
+                raise ValueError("h_out takes bf16 rows: MXFP4 rows are allocated by the call")
+            h = MXFP4Rows._unwritten(rows, C, x.device)
+            hp, ldh, hdt, hsp = h.qp, h.ldq, FW_DT_MXFP4, h.sp
         else:
-            h, hp, ldh, hdt, hsp = mx, mx.qp, mx.ldq, FW_DT_MXFP4, mx.sp
+            h, ldh, hdt, hsp = h_out, C, FW_DT_BF16, 0
+            if h is None:
+                h = torch.empty((rows, C), dtype=torch.bfloat16, device=x.device)
+            else:
+                ldh = self._rows("h_out", h, torch.bfloat16)
+                if h.shape != x.shape:
+                    raise ValueError(f"h_out: x's shape {tuple(x.shape)} expected, got {tuple(h.shape)}")
+            hp = h.data_ptr()
         _check(self.lib.fw_residual_norm(
             x.data_ptr(), ldx, xop, ldxo, _dt(x), yp, ldy, ydt, ptrs[0], ptrs[1], ptrs[2], post, ptrs[3], RNORM[norm], ptrs[4], ptrs[5], ptrs[6], ptrs[7], eps,
             hp, ldh, hdt, hsp, rows, C, max(1, rows // (groups or 1)), st), "fw_residual_norm")

@@ -212,8 +212,9 @@ def install(model, ops=None, device=None, cache_step_invariants=True, precision=
     """Replace `model.joint_forward` by the MI355X engine.  `ops` defaults to HipOps (raises without a GPU / library);
     tests may inject another op set to exercise this boundary on CPU.  `cache_step_invariants`: keep the context embeddings,
     the per-block cross-attention K/V and the camera adapter's Pluecker term across the calls of a generation (the caller
-    passes the same tensors 100 times; results are bit-identical).  `precision`: "bf16", or "fp8" = the
-    DiT blocks' linears through the reference's fp8 linear.  `fp8_attention=True` (with precision="fp8":
+    passes the same tensors 100 times; results are bit-identical).  `precision`: "bf16", "fp8" = the
+    DiT blocks' linears through the reference's fp8 linear, or "mxfp4" = the same linears with weights and inputs in
+    MXFP4, an option without reference semantics.  `fp8_attention=True` (with precision="fp8":
     BASELINE config 5, "fp8 attention + FFN"): the DiT self-attention on e4m3 q / k / v / probabilities as well.  The reference
     defines fp8 for nn.Linear only, so this option has NO reference semantics to be exact against: its stated, test-enforced
     tolerance is 2e-2 rel-L2 of noise_pred against the same engine with bf16 attention (measured 1.35e-2 at 40 / 24 / 24 blocks,

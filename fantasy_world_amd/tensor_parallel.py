@@ -35,7 +35,7 @@ LayerScale / residual epilogue runs after the reduction (fw_residual_add).  Over
 import torch
 import torch.distributed as dist
 
-from .engine import FusionEngine, _DitBlock, _VggtBlock, _Bicross, _pad_to, _ru64
+from .engine import PRECISIONS, FusionEngine, _DitBlock, _VggtBlock, _Bicross, _pad_to, _ru64
 from .parallel import Pending, Ready, split_counts
 
 
@@ -121,9 +121,11 @@ class TPFusionEngine(FusionEngine):
         per-row scale_a of layers.py:126-133 is a property of the FULL row: the local row maxima are all-reduced (MAX, fp32 [rows]:
         131 KB at L = 32 760) BEFORE quantising, so every rank divides by the same scale (fw_row_absmax, fw_fp8_quant_rows_amax);
         the partial products (x scale_a, no bias) are all-reduced like the bf16 ones and the e4m3-rounded bias rides in the
-        epilogue after the reduction.  fp8_attention: this rank's heads through fw_attention_fp8."""
-        if precision not in ("bf16", "fp8"):
-            raise ValueError(f"precision must be 'bf16' or 'fp8', got {precision!r}")
+        epilogue after the reduction.  fp8_attention: this rank's heads through fw_attention_fp8.
+        precision="mxfp4": a block scale belongs to 32 neighbouring values of a row, and every rank's K-slice (heads of 128, FFN units of
+        64) starts and ends on a block: slices of the quantised row are the quantised slices, so nothing is exchanged for it."""
+        if precision not in PRECISIONS:
+            raise ValueError(f"precision must be one of {PRECISIONS}, got {precision!r}")
         for name, H in (("DiT", cfg.num_heads), ("VGGT", cfg.vggt_heads)):
             if not tp.divides(H):
                 raise ValueError(f"{H} {name} heads do not divide over {tp.world} tensor-parallel ranks")
@@ -142,7 +144,8 @@ class TPFusionEngine(FusionEngine):
         c0, c1 = h0 * hd, h1 * hd
         f8 = self.precision == "fp8"           # the DiT block's nn.Linear modules (engine.py _pack_dit): q/k/v/o of both attentions, FFN
         pk = lambda w, bias=None: ops.pack_linear(w, bias)
-        pk8 = (lambda w, bias=None: ops.pack_linear(w, bias, fp8=True)) if f8 else pk
+        kind = self._linear_kind()
+        pk8 = lambda w, bias=None: ops.pack_linear(w, bias, **kind)
         # a row-parallel linear's bias is applied AFTER the reduction (fw_residual_add): under fp8 it is the value the fp8 linear
         # adds -- rounded to bf16 and, inside AutoWrappedLinear, through e4m3 (layers.py:138,158-159)
         rbias = (lambda n: ops.fp8_bias(g(n))) if f8 else (lambda n: ops.to_f32(g(n)))
@@ -234,9 +237,11 @@ class TPFusionEngine(FusionEngine):
         return bc
 
     # ------------------------------------------------------------------------------------------------ helpers
-    def _reduce_into(self, stream, x_in, lin, bias, g1=None, g0=None, kind="all_reduce"):
+    def _reduce_into(self, stream, x_in, lin, bias, g1=None, g0=None, kind="all_reduce", norm=None):
         """stream += (all_reduce(x_in @ lin^T) + bias) * g1 + g0, as a generator: row blocks so that the reduction of block c flies
-        behind the GEMM of block c+1 (and behind whatever the interleaved branch enqueues at the yield)."""
+        behind the GEMM of block c+1 (and behind whatever the interleaved branch enqueues at the yield).
+        norm (layernorm's keywords): what follows is that LayerNorm of the stream and nothing else touches the stream in between -- the
+        update and the norm are one pass (residual_norm: the bits of residual_add, then layernorm), and its rows are returned."""
         ops, tp = self.ops, self.tp
         M = x_in.shape[0]
         nch = max(1, min(tp.chunks, M // tp.chunk_rows)) if tp.world > 1 else 1
@@ -255,8 +260,13 @@ class TPFusionEngine(FusionEngine):
             part = ops.linear(rows_of(a, b), lin, out_f32=f32)
             pend.append((a, b, tp.all_reduce_async(part, kind)))
         yield
+        h = None if norm is None else ops.empty(M, stream.shape[1])
         for a, b, p in pend:
-            ops.residual_add(stream[a:b], p.wait(), bias=bias, g1=g1, g0=g0)
+            if norm is None:
+                ops.residual_add(stream[a:b], p.wait(), bias=bias, g1=g1, g0=g0)
+            else:
+                ops.residual_norm(stream[a:b], p.wait(), bias=bias, g1=g1, g0=g0, h_out=h[a:b], **norm)
+        return h
 
     def _stats(self, *slices):
         """Sum of squares over the FULL width of each row for several (rows, local-columns) slices: one fused all-reduce."""
@@ -269,15 +279,16 @@ class TPFusionEngine(FusionEngine):
         return tp.all_reduce_async(buf, "all_reduce_stats"), outs
 
     # ------------------------------------------------------------------------------------------------ blocks (generators)
-    def _tp_dit_attn(self, blk, x, ctx_txt, ctx_img, t_mod, tabs, plucker, out):
-        """Self-attention + cross-attention (+ camera adapter) of one DiT block; out["mod"] receives the modulation table."""
+    def _tp_dit_attn(self, blk, x, ctx_txt, ctx_img, t_mod, tabs, plucker, out, then_ffn=False):
+        """Self-attention + cross-attention (+ camera adapter) of one DiT block; out["mod"] receives the modulation table.  then_ffn: the
+        block's FFN half follows directly; out["xn"] receives its normalised rows."""
         cfg, ops, tp = self.cfg, self.ops, self.tp
         D, hd = cfg.dim, cfg.head_dim
         Hl = cfg.num_heads // tp.world
         W = Hl * hd
         h0 = tp.heads(cfg.num_heads)[0]
         mod = out["mod"] = self._dit_mod(blk, t_mod)
-        xn = ops.layernorm(x, scale=mod[1], shift=mod[0], eps=cfg.eps)
+        xn = self._norm_into(blk.qkv, x, scale=mod[1], shift=mod[0], eps=cfg.eps)
         qkv = ops.linear(xn, blk.qkv)                                   # [L, 3 W]: this rank's heads
         q, k, v = qkv[:, :W], qkv[:, W:2 * W], qkv[:, 2 * W:]
         pend, (sq, sk) = self._stats(q, k)
@@ -298,9 +309,8 @@ class TPFusionEngine(FusionEngine):
             ops.qk_prep(k, Hl, hd, norm="rms_full", norm_w=blk.norm_k, eps=cfg.eps, rope="interleaved", table=tab,
                         ext_sumsq=sk, norm_width=D)
             o = ops.attention(q, k, v, Hl, hd, batch=1, q_prescaled=True)
-        yield from self._reduce_into(x, o, blk.o, blk.o_b, g1=mod[2])
         # cross-attention: text + image keys share q (wan_video_dit.py:185-201)
-        xn3 = ops.layernorm(x, w=blk.norm3_w, b=blk.norm3_b, eps=cfg.eps)
+        xn3 = yield from self._reduce_into(x, o, blk.o, blk.o_b, g1=mod[2], norm=dict(w=blk.norm3_w, b=blk.norm3_b, eps=cfg.eps))
         qc = ops.linear(xn3, blk.cq)
         kv = ops.linear(ctx_txt, blk.ckv)
         sl = [qc, kv[:, :W]]
@@ -327,15 +337,16 @@ class TPFusionEngine(FusionEngine):
             comb = ops.linear(t1, blk.a_g22, res=pterm, out=pterm)
             t2 = ops.linear(comb, blk.a_v0, act="relu")
             ops.linear(t2, blk.a_v2, res=oc, out=oc)                    # my columns of the shift
-        yield from self._reduce_into(x, oc, blk.co, blk.co_b)
+        out["xn"] = yield from self._reduce_into(x, oc, blk.co, blk.co_b, norm=dict(scale=mod[4], shift=mod[3], eps=cfg.eps) if then_ffn else None)
 
-    def _tp_dit_ffn(self, blk, x, mod):
+    def _tp_dit_ffn(self, blk, x, mod, xn=None):
         cfg, ops = self.cfg, self.ops
-        xn = ops.layernorm(x, scale=mod[4], shift=mod[3], eps=cfg.eps)
+        if xn is None:
+            xn = self._norm_into(blk.ffn0, x, scale=mod[4], shift=mod[3], eps=cfg.eps)
         h = ops.linear(xn, blk.ffn0, act="gelu_tanh")                   # [L, Fd / n]
         yield from self._reduce_into(x, h, blk.ffn2, blk.ffn2_b, g1=mod[5])
 
-    def _tp_vggt_attn(self, blk, tok, e0, tabs, batch, out):
+    def _tp_vggt_attn(self, blk, tok, e0, tabs, batch, out, then_mlp=False):
         cfg, ops, tp = self.cfg, self.ops, self.tp
         C = cfg.vggt_dim
         hd = C // cfg.vggt_heads
@@ -350,11 +361,13 @@ class TPFusionEngine(FusionEngine):
         ops.qk_prep(k, Hl, hd, norm="ln_head", norm_w=blk.k_norm[0], norm_b=blk.k_norm[1], eps=cfg.vggt_eps, rope="half2d",
                     table=tabs["vggt"])
         o = ops.attention(q, k, v, Hl, hd, batch=batch, q_prescaled=True)
-        yield from self._reduce_into(tok, o, blk.proj, blk.proj_b, g1=blk.ls1)
+        out["xn"] = yield from self._reduce_into(tok, o, blk.proj, blk.proj_b, g1=blk.ls1,
+                                                 norm=dict(w=blk.norm2[0], b=blk.norm2[1], eps=cfg.vggt_eps) if then_mlp else None)
 
-    def _tp_vggt_mlp(self, blk, tok, e):
+    def _tp_vggt_mlp(self, blk, tok, e, xn=None):
         cfg, ops = self.cfg, self.ops
-        xn = ops.layernorm(tok, w=blk.norm2[0], b=blk.norm2[1], eps=cfg.vggt_eps)
+        if xn is None:
+            xn = ops.layernorm(tok, w=blk.norm2[0], b=blk.norm2[1], eps=cfg.vggt_eps)
         h = ops.linear(xn, blk.fc1, act="gelu_erf")
         g1, g0 = self._vggt_gates(blk, e)
         yield from self._reduce_into(tok, h, blk.fc2, blk.fc2_b, g1=g1, g0=g0)
@@ -415,8 +428,8 @@ class TPFusionEngine(FusionEngine):
 
         for b in range(cfg.start_index):
             blk, sd = self.dit[b], {}
-            _drain(self._tp_dit_attn(blk, xs, ctx_txt, ctx_img, t_mod, tabs, plucker, sd))
-            _drain(self._tp_dit_ffn(blk, xs, sd["mod"]))
+            _drain(self._tp_dit_attn(blk, xs, ctx_txt, ctx_img, t_mod, tabs, plucker, sd, then_ffn=True))
+            _drain(self._tp_dit_ffn(blk, xs, sd["mod"], sd["xn"]))
             if per_block is not None:
                 per_block("x", b, xs)
         if collect is not None:
@@ -434,8 +447,8 @@ class TPFusionEngine(FusionEngine):
 
             def vggt_branch():
                 # frame block (attention + MLP), then the global block's attention half (aggregator.py:215-260, block.py:59-69)
-                yield from self._tp_vggt_attn(fb, tok, e0, tabs, F, sf)
-                yield from self._tp_vggt_mlp(fb, tok, sf["e"])
+                yield from self._tp_vggt_attn(fb, tok, e0, tabs, F, sf, then_mlp=True)
+                yield from self._tp_vggt_mlp(fb, tok, sf["e"], sf.pop("xn"))
                 if i in need:
                     sf["frame_out"] = tok.clone()
                 yield from self._tp_vggt_attn(gb, tok, e0, tabs, 1, sg)

@@ -18,9 +18,23 @@ import torch.nn.functional as F
 class _Lin:
     __slots__ = ("w", "b", "N", "K", "fp8")
 
+    mxfp4 = False
+
     def __init__(self, w, b, fp8=False):
         self.w, self.b, self.fp8 = w, b, fp8
         self.N, self.K = w.shape
+
+
+class _MXRows:
+    """What MXFP4 rows stand for, in fp32 [M, K]."""
+
+    def __init__(self, v):
+        self.v, self.shape = v, v.shape
+
+
+class _MXLin(_Lin):
+    __slots__ = ()
+    mxfp4 = True
 
 
 class TorchRefOps:
@@ -65,10 +79,12 @@ class TorchRefOps:
     def to_act(self, t):
         return self._r(t.detach().to(device=self.device, dtype=torch.float32), "input").contiguous()
 
-    def pack_linear(self, w, b, fp8=False):
+    def pack_linear(self, w, b, fp8=False, mxfp4=False):
         assert w.shape[1] % 64 == 0
         if fp8:
             return self.pack_linear_fp8(w, b)
+        if mxfp4:
+            return self.pack_linear_mxfp4(w, b)
         return _Lin(self._r(self.to_f32(w), "weight"), None if b is None else self.to_f32(b))
 
     def pack_linear_f32(self, w, b):
@@ -89,8 +105,12 @@ class TorchRefOps:
             return F.silu(y)
         raise ValueError(act)
 
-    def linear(self, x, lin, act=None, g1=None, g0=None, res=None, out_f32=False, out=None):
-        if lin.fp8:      # fp8_linear (layers.py:115-151) by its definition, then the same epilogue
+    def linear(self, x, lin, act=None, g1=None, g0=None, res=None, out_f32=False, out=None, out_mxfp4=False):
+        if lin.mxfp4:    # both operands in MXFP4 by the definition; the rows' bf16 rounding first, as the HIP path's inputs are bf16
+            v = x.v if isinstance(x, _MXRows) else self._mx(x.to(torch.bfloat16).float())
+            assert v.shape[1] == lin.K
+            y = (v.double() @ lin.w.double().t()).float()
+        elif lin.fp8:      # fp8_linear (layers.py:115-151) by its definition, then the same epilogue
             q, scale = x if isinstance(x, tuple) else self.quantize_fp8_rows(x)      # (rows already quantised, their scale)
             assert q.shape[1] == lin.K
             # e4m3 x e4m3 products summed in fp64: exact, so the result does not depend on how M / N / K are blocked or sharded
@@ -107,6 +127,8 @@ class TorchRefOps:
             y = y + g0
         if res is not None:
             y = y + res
+        if out_mxfp4:
+            return _MXRows(self._mx(y.to(torch.bfloat16).float()))
         if not out_f32:
             y = self._r(y, f"linear_out:N{lin.N}:K{lin.K}")
         if out is not None:
@@ -405,6 +427,33 @@ class TorchRefOps:
 
     def activation(self, x, act):
         return self._r(self._act(x.to(torch.float32), act))
+
+    # ---- MXFP4 (include/fw_mi355x.h: encoding rule) ------------------------------------------------------------------------------
+    @staticmethod
+    def _mx(x):
+        """MXFP4 of the rows of x (finite values), as the fp32 values the codes stand for."""
+        M, K = x.shape
+        v = F.pad(x.double(), (0, -K % 32)).view(M, -1, 32)
+        m, e = torch.frexp(v.abs().amax(-1, keepdim=True))
+        unit = torch.exp2((e - 3 + (m >= 0.875)).clamp(-127, 125).double())
+        a = v / unit
+        step = torch.where(a.abs() < 2, 0.5, torch.where(a.abs() < 4, 1.0, 2.0)).double()
+        return ((torch.round(a / step) * step).clamp(-6, 6) * unit).view(M, -1)[:, :K].float()
+
+    def pack_linear_mxfp4(self, w, b):
+        return _MXLin(self._mx(self.to_f32(w)), None if b is None else self.to_f32(b))
+
+    def residual_norm(self, x, y=None, bias=None, g1=None, g0=None, w=None, b=None, scale=None, shift=None, eps=1e-6, out="bf16", h_out=None):
+        """fw_residual_norm in the engine's use of it (LayerNorm, no post norm, in place): residual_add, then layernorm."""
+        if y is not None:
+            self.residual_add(x, y, bias=bias, g1=g1, g0=g0)
+        h = self.layernorm(x, w=w, b=b, scale=scale, shift=shift, eps=eps)
+        if out == "mxfp4":
+            return _MXRows(self._mx(h.to(torch.bfloat16).float()))
+        if h_out is not None:
+            h_out.copy_(h)
+            return h_out
+        return h
 
     # ---- fp8 linear (SURVEY.md A19) ----------------------------------------------------------------------------------------
     def pack_linear_fp8(self, w, b, bias_through_fp8=True):
