@@ -15,6 +15,7 @@ Other workloads (never the headline; `config.workload` names them):
                                                 expert chosen per step (inference_wan22.py:229-277)
     --precision fp8                             BASELINE configs[4]'s arithmetic: the DiT blocks' linears through the fp8 linear
                                                 (diffsynth_wan22/vram_management/layers.py:115-151); `dtype` says "fp8_e4m3"
+    --precision mxfp4                           the same linears with weights and inputs in MXFP4 (an option without reference semantics)
     --merge-cfg                                 N = 1: both CFG passes of a step as one forward over 2L rows
     --cache-invariants                          step-invariant intermediates cached; off = the
                                                 reference's per-step work
@@ -42,6 +43,7 @@ if ROOT not in sys.path:
 
 MFMA_BF16_PEAK = 2.5e15      # dense bf16 MFMA peak, /opt/skills/guides/MI355X_MICROARCH.md chip table
 MFMA_FP8_PEAK = 5.0e15       # dense fp8 MFMA peak, same table
+MFMA_FP4_PEAK = 10.0e15      # dense fp4 MFMA peak (twice fp8)
 
 # PREDICTED step time (ms, best .. worst) of the HEADLINE workload per (N, partition), communication included -- tools/predict_scaling.py,
 # profiles/r05/scaling_prediction.txt: one-GPU shard emulation + counted bytes / assumed xGMI link rates.  NOT a measurement: printed
@@ -80,7 +82,7 @@ def parse_args(argv=None):
     ap.add_argument("--height", type=int, default=480)
     ap.add_argument("--width", type=int, default=832)
     ap.add_argument("--layers", type=int, default=40, help="debug only: anything but 40 is not a BASELINE workload")
-    ap.add_argument("--precision", choices=["bf16", "fp8"], default="bf16")
+    ap.add_argument("--precision", choices=["bf16", "fp8", "mxfp4"], default="bf16")
     ap.add_argument("--fp8-attention", action="store_true",
                     help="with --precision fp8: the DiT self-attention on e4m3 q / k / v / probabilities too (BASELINE configs[4]: "
                          "'fp8 attention + FFN'; parity unpinned -- the reference defines no fp8 attention; never the headline)")
@@ -446,7 +448,7 @@ def main():
     f_fwd = forward_flops(cfg, L, L2, F, P, 512, Li)
     step_flops = 2.0 * f_fwd
     value = args.steps / dt
-    peak = MFMA_FP8_PEAK if args.precision == "fp8" else MFMA_BF16_PEAK
+    peak = {"fp8": MFMA_FP8_PEAK, "mxfp4": MFMA_FP4_PEAK}.get(args.precision, MFMA_BF16_PEAK)
     # dominant kernel: one hd-128 self-attention launch = 4 * Lq_local * L * D FLOP (QK^T + PV)
     # (sharded: L rows x 40/n heads per rank after the head exchange = the same FLOPs as L/n rows x 40 heads; a block's heads
     #  go through the kernel in groups under the shard (FusionEngine._head_groups): average per launch)
@@ -475,6 +477,8 @@ def main():
                          "frac_of_bf16_peak": None if fl is None else fl / (ms * 1e-3) / MFMA_BF16_PEAK}
         if args.precision == "fp8" and name.startswith("gemm_") and fl is not None:
             kernels[name]["frac_of_fp8_peak"] = fl / (ms * 1e-3) / MFMA_FP8_PEAK      # the DiT blocks' linears run e4m3 x e4m3
+        if args.precision == "mxfp4" and name.startswith("gemm_") and fl is not None:
+            kernels[name]["frac_of_fp4_peak"] = fl / (ms * 1e-3) / MFMA_FP4_PEAK
         if name.startswith("attn_hd") and fl is not None and "cross" not in name:
             kernels[name]["matrix_pipe"] = attention_measured(int(name[7:].split("_")[0]))
     # HBM-side traffic of the dominant kernel: measured with rocprofv3 PMC counters in separate passes (FETCH_SIZE, WRITE_SIZE)
@@ -510,7 +514,8 @@ def main():
         "dtype": ("fp8_e4m3 linears (fp32 accumulate), " + (("fp8_e4m3 DiT self-attention" + (" and bicross attention" if getattr(eng, "fp8_bicross", False) else "") + (" and VGGT frame / global attention" if getattr(eng, "fp8_vggt", False) else "")
                                                            + " (fp32 scores / softmax / accumulate; parity unpinned)")
                                                           if fp8_attn else "bf16 attention"))
-                 if args.precision == "fp8" else "bf16", "data": "synthetic",
+                 if args.precision == "fp8" else ("mxfp4 linears (fp32 accumulate), " + ("fp8_e4m3" if fp8_attn else "bf16") + " DiT self-attention; no reference semantics")
+                 if args.precision == "mxfp4" else "bf16", "data": "synthetic",
         "config": {"workload": workload, "dit_tokens": L, "vggt_tokens": L2, "cfg_forwards_per_step": 2,
                    "parallelism": topo.describe(), "step_invariant_cache": bool(args.cache_invariants),
                    "cfg_merged_in_one_pass": bool(args.merge_cfg and world == 1),
