@@ -470,9 +470,9 @@ __global__ __launch_bounds__(512, 2) void gemm_mxfp4_256_kernel(MxArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Up to 16 rows: the weights are all there is to read, so the split is made for them.  A work-group takes 16 NB columns (W rows) and all
-// rows of A, its 8 waves a run of K each, v_mfma_scale_f32_16x16x128_f8f6f4 (lane l: row l & 15, block l >> 4 of four); a wave requests all
-// W of eight instructions before it multiplies, which keeps the whole matrix in flight across the chip.  The eight partial sums are added
+// Up to 32 rows: the weights are all there is to read, so the split is made for them.  A work-group takes 16 NB columns (W rows) and all
+// rows of A (16 MT), its 8 waves a run of K each, v_mfma_scale_f32_16x16x128_f8f6f4 (lane l: row l & 15, block l >> 4 of four); a wave requests all
+// W of its next 2 to 8 instructions (UB) before it multiplies, which keeps the whole matrix in flight across the chip.  The eight partial sums are added
 // in LDS, in wave order: no atomics, no workspace, the same bits every time.
 // FUSED: A is bf16 and the work-group quantises all of it into LDS, a block of 32 a lane, while its first W is on the way;
 // every work-group repeats that, which costs less than a launch and a round trip through memory.  LDS rows are padded by one 16-byte chunk,
@@ -481,10 +481,10 @@ __global__ __launch_bounds__(512, 2) void gemm_mxfp4_256_kernel(MxArgs p) {
 #define FWX_MFMA16(A, B, C, SA, SB) __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( \
     i32x8_t{(A)[0], (A)[1], (A)[2], (A)[3], 0, 0, 0, 0}, i32x8_t{(B)[0], (B)[1], (B)[2], (B)[3], 0, 0, 0, 0}, C, 4, 4, 0, SA, 0, SB)
 
-template <int NB, bool FUSED>
+template <int MT, int NB, bool FUSED>
 __global__ __launch_bounds__(512, 4) void gemm_mxfp4_rows_kernel(MxArgs p, int blocks) {
-    constexpr int UB = NB == 1 ? 8 : 4;              // instructions (of 128 values of K) whose operands are requested together
-    __shared__ float red[8][NB * 4][64];
+    constexpr int UB = MT * NB == 1 ? 8 : NB == 4 ? 2 : 4;      // instructions (of 128 values of K) whose operands are requested together
+    __shared__ float red[8][MT * NB * 4][64];
     extern __shared__ u32x4_t mx_rows[];                  // FUSED: codes [M][slabs * 8 + 1] chunks, then scale bytes [M][slabs * 8]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, h = lane >> 4;
@@ -501,14 +501,19 @@ __global__ __launch_bounds__(512, 4) void gemm_mxfp4_rows_kernel(MxArgs p, int b
     }
     const int chunks = p.slabs * 8;                       // 16-byte chunks = blocks of a padded row
     uint8_t* smem_s = (uint8_t*)(mx_rows + p.M * (chunks + 1));
-    const int arow = min(r, p.M - 1);
-    const uint8_t* ap = FUSED ? (const uint8_t*)(mx_rows + arow * (chunks + 1) + h) : p.A + (int64_t)arow * p.lda + h * 16;
-    const uint8_t* sap = FUSED ? smem_s + arow * chunks + h : p.sa + arow * 8 + h;
-    f32x4_t acc[NB];
+    const uint8_t* ap[MT];
+    const uint8_t* sap[MT];
+    f32x4_t acc[MT][NB];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) acc[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    i32x4_t w[UB][NB], a[UB];
-    int sw[UB][NB], sa[UB];
+    for (int m = 0; m < MT; ++m) {
+        const int row = min(m * 16 + r, p.M - 1);
+        ap[m] = FUSED ? (const uint8_t*)(mx_rows + row * (chunks + 1) + h) : p.A + (int64_t)row * p.lda + h * 16;
+        sap[m] = FUSED ? smem_s + row * chunks + h : p.sa + row * 8 + h;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[m][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    i32x4_t w[UB][NB], a[UB][MT];
+    int sw[UB][NB], sa[UB][MT];
     auto load_w = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < UB; ++i)
@@ -544,26 +549,34 @@ __global__ __launch_bounds__(512, 4) void gemm_mxfp4_rows_kernel(MxArgs p, int b
 #pragma unroll
         for (int i = 0; i < UB; ++i)
             if (u + i < u1) {
-                a[i] = *(const i32x4_t*)(ap + (int64_t)(u + i) * 64);
-                sa[i] = FUSED ? sap[(u + i) * 4] : sap[(int64_t)((u + i) >> 1) * 256 + ((u + i) & 1) * 4];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    a[i][m] = *(const i32x4_t*)(ap[m] + (int64_t)(u + i) * 64);
+                    sa[i][m] = FUSED ? sap[m][(u + i) * 4] : sap[m][(int64_t)((u + i) >> 1) * 256 + ((u + i) & 1) * 4];
+                }
             }
 #pragma unroll
         for (int i = 0; i < UB; ++i)
             if (u + i < u1) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) acc[b] = FWX_MFMA16(a[i], w[i][b], acc[b], sa[i], sw[i][b]);
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) acc[m][b] = FWX_MFMA16(a[i][m], w[i][b], acc[m][b], sa[i][m], sw[i][b]);
             }
     }
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[wave][b * 4 + i][lane] = acc[b][i];
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) red[wave][(m * NB + b) * 4 + i][lane] = acc[m][b][i];
     __syncthreads();
     // lane l of a fragment holds column l & 15 of rows 4 (l >> 4) .. + 3
     constexpr int COLS = 16 * NB;
-    if (threadIdx.x < 16 * COLS) {                        // whole waves
-        const int row = threadIdx.x / COLS, c = threadIdx.x % COLS, col = n0 + c;
-        const int slot = (c >> 4) * 4 + (row & 3), at = (row >> 2) * 16 + (c & 15);
+#pragma unroll
+    for (int e = threadIdx.x; e < 16 * MT * COLS; e += 512) {      // whole waves: 256, 512 or 1024 results
+        const int row = e / COLS, c = e % COLS, col = n0 + c;
+        const int slot = ((row >> 4) * NB + (c >> 4)) * 4 + (row & 3), at = ((row >> 2) & 3) * 16 + (c & 15);
         float v = red[0][slot][at];
 #pragma unroll
         for (int k = 1; k < 8; ++k) v += red[k][slot][at];
@@ -575,7 +588,7 @@ __global__ __launch_bounds__(512, 4) void gemm_mxfp4_rows_kernel(MxArgs p, int b
             const int64_t o = (int64_t)row * p.ldr + col;
             v += p.res_dtype == FW_DT_F32 ? ((const float*)p.res)[o] : bf16_bits_to_f32(((const uint16_t*)p.res)[o]);
         }
-        if (NB == 2 && p.out_dtype == FW_DT_MXFP4) {      // 32 lanes hold a block
+        if (NB > 1 && p.out_dtype == FW_DT_MXFP4) {      // 32 lanes hold a block
             const uint32_t b16 = in ? f32_to_bf16_bits(v) : 0;
             uint32_t top = (b16 & 0x7fffu) << 16;
 #pragma unroll
@@ -586,7 +599,7 @@ __global__ __launch_bounds__(512, 4) void gemm_mxfp4_rows_kernel(MxArgs p, int b
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) q |= (uint32_t)__shfl_xor((int)q, o, 64);
             if (live && (c & 7) == 0) *(uint32_t*)((uint8_t*)p.C + (int64_t)row * p.ldc + (col >> 1)) = q;
-            if (live && c == 0) p.cs[((int64_t)(row >> 5) * p.cslabs + (col >> 8)) * 256 + (row & 31) * 8 + ((col >> 5) & 7)] = (uint8_t)byte;
+            if (live && (c & 31) == 0) p.cs[((int64_t)(row >> 5) * p.cslabs + (col >> 8)) * 256 + (row & 31) * 8 + ((col >> 5) & 7)] = (uint8_t)byte;
         } else if (live && in) {
             const int64_t o = (int64_t)row * p.ldc + col;
             if (p.out_dtype == FW_DT_F32) ((float*)p.C)[o] = v;
@@ -626,18 +639,26 @@ int mx_tile_choice(int M, int n_cover, int slabs) {
     return best;
 }
 
-template <bool FUSED>
+// Columns of a work-group: as few as give every CU one (16 NB, the whole K each), then wider rather than a second round.  Same bits each.
+//     us, NB = 1 / 2 / 4     1 x 5120 x 5120    16 x 5120 x 5120    32 x 4096 x 1024    16 x 13824 x 5120    16 x 30000 x 2048
+//     from MXFP4 rows         5.4 / 5.5 / 8.5     7.5 / 6.2 / 9.4     3.0 / 3.6 / 5.0    14.0 / 11.1 / 10.5    14.0 / 10.2 / 8.9
+//     from bf16 rows          5.5 / 5.6 / 8.1    11.3 / 9.0 / 12.0    4.1 / 4.7 / 6.2    21.2 / 16.0 / 13.4    18.9 / 13.2 / 10.8
+template <int MT, bool FUSED>
 int mx_launch_rows(const MxArgs& p, int n_cover, int blocks, hipStream_t st) {
     const int lds = FUSED ? p.M * (p.slabs * 8 + 1) * 16 + p.M * p.slabs * 8 : 0;
-    if (p.out_dtype == FW_DT_MXFP4) hipLaunchKernelGGL((gemm_mxfp4_rows_kernel<2, FUSED>), dim3((unsigned)((n_cover + 31) / 32)), dim3(512), lds, st, p, blocks);
-    else hipLaunchKernelGGL((gemm_mxfp4_rows_kernel<1, FUSED>), dim3((unsigned)((n_cover + 15) / 16)), dim3(512), lds, st, p, blocks);
+    int nb = p.out_dtype == FW_DT_MXFP4 ? 2 : 1;
+    while (nb < 4 && n_cover > 256 * 16 * nb) nb *= 2;
+    const dim3 grid((unsigned)((n_cover + 16 * nb - 1) / (16 * nb)));
+    if (nb == 4) hipLaunchKernelGGL((gemm_mxfp4_rows_kernel<MT, 4, FUSED>), grid, dim3(512), lds, st, p, blocks);
+    else if (nb == 2) hipLaunchKernelGGL((gemm_mxfp4_rows_kernel<MT, 2, FUSED>), grid, dim3(512), lds, st, p, blocks);
+    else hipLaunchKernelGGL((gemm_mxfp4_rows_kernel<MT, 1, FUSED>), grid, dim3(512), lds, st, p, blocks);
     return (int)hipGetLastError();
 }
 
-// Rows that fw_linear_mxfp4 quantises inside the product: at most 16, in whole 16-byte accessible blocks, that take at most 48 KiB of LDS
-// (two work-groups of 8 waves a CU; 16 x 5120 takes 44)
+// Rows that fw_linear_mxfp4 quantises inside the product: at most 32, in whole 16-byte accessible blocks, that take at most 48 KiB of LDS.
+// 21 x 4096 x 1024: 3.6 us, in two launches 8.3; 16 x 5120 x 5120: 9.0, in two launches 9.3 -- and 3 us less of the host's time each.
 bool mx_rows_fused(const void* x, int64_t ldx, int M, int K) {
-    return M <= 16 && K > 0 && (K % 32) == 0 && (ldx % 8) == 0 && (((uintptr_t)x) & 15) == 0 && (int64_t)M * (mx_slabs(K) * 136 + 16) <= 48 * 1024;
+    return M <= 32 && K > 0 && (K % 32) == 0 && (ldx % 8) == 0 && (((uintptr_t)x) & 15) == 0 && (int64_t)M * (mx_slabs(K) * 136 + 16) <= 48 * 1024;
 }
 
 }  // namespace
@@ -680,7 +701,8 @@ extern "C" int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, c
     p.A = A; p.lda = lda; p.sa = sa;
     const int n_cover = out_dtype == FW_DT_MXFP4 ? cslabs * MX_SLAB : N;       // the padding of a quantised row is written too
     hipStream_t st = (hipStream_t)stream;
-    if (M <= 16) return mx_launch_rows<false>(p, n_cover, 0, st);      // 16 x 5120 x 5120: 7.6 us, the 64 x 128 tiles 9.7; the same kernel for 32 rows took 10.4
+    if (M <= 16) return mx_launch_rows<1, false>(p, n_cover, 0, st);
+    if (M <= 32) return mx_launch_rows<2, false>(p, n_cover, 0, st);
     int choice = mx_tile_choice(M, n_cover, slabs);
     if (choice == 3) {
         // a tail of at most 128 rows past the last full tile does not get a round of 256-row tiles: it goes by the same rule on its own
@@ -723,7 +745,8 @@ extern "C" int fw_linear_mxfp4(const uint16_t* x, int64_t ldx, const uint8_t* W,
         MxArgs p;
         if (const int rc = mx_args(p, W, ldw, sw, C, ldc, out_dtype, cs, M, N, K, bias, act, g1, g0, res, ldr, res_dtype)) return rc;
         p.A = (const uint8_t*)x; p.lda = ldx * 2; p.sa = nullptr;
-        return mx_launch_rows<true>(p, out_dtype == FW_DT_MXFP4 ? p.cslabs * MX_SLAB : N, K / 32, (hipStream_t)stream);
+        const int n_cover = out_dtype == FW_DT_MXFP4 ? p.cslabs * MX_SLAB : N;
+        return M <= 16 ? mx_launch_rows<1, true>(p, n_cover, K / 32, (hipStream_t)stream) : mx_launch_rows<2, true>(p, n_cover, K / 32, (hipStream_t)stream);
     }
     if (!workspace || workspace_bytes < fw_linear_mxfp4_workspace_bytes(M, K) || (((uintptr_t)workspace) & 15)) {
         fw_set_error("fw_linear_mxfp4: a 16-byte aligned workspace of fw_linear_mxfp4_workspace_bytes(M, K) required"); return FW_E_BADARG; }

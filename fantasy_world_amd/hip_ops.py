@@ -748,7 +748,7 @@ class HipOps:
     # ---- MXFP4 linear (include/fw_mi355x.h; no reference semantics) ------------------------------------------------------------------
     def _enter(self, *tensors):
         """The current stream, for a call whose tensors all lie on the current device (and on the one this object is bound to)."""
-        dev = torch.cuda.current_device()
+        dev = torch._C._cuda_getDevice()
         if self.device.index is not None and dev != self.device.index:
             raise RuntimeError(f"HipOps bound to {self.device} but the current HIP device is {dev}: call torch.cuda.set_device(...) (one process per GPU)")
         for t in tensors:
@@ -759,16 +759,13 @@ class HipOps:
     @staticmethod
     def _rows(name, t, *dtypes):
         """t [rows, width], one of dtypes, contiguous inside a row; -> its row stride (at least the width, where there is at most one row)."""
-        if t.dim() != 2 or t.dtype not in dtypes or t.shape[1] < 1 or (t.stride(1) != 1 and t.shape[1] > 1):
-            raise ValueError(f"{name}: rows of {dtypes} expected, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
-        ld = t.stride(0)
-        return ld if ld >= t.shape[1] else HipOps._short(name, t)
-
-    @staticmethod
-    def _short(name, t):
-        if t.shape[0] > 1:
-            raise ValueError(f"{name}: rows overlap, shape {tuple(t.shape)} with strides {t.stride()}")
-        return t.shape[1]
+        if t.dim() != 2 or t.dtype not in dtypes:
+            raise ValueError(f"{name}: rows of {dtypes} expected, got {t.dtype} {tuple(t.shape)}")
+        ld, one = t.stride()
+        width = t.size(1)
+        if width < 1 or (one != 1 and width > 1) or (ld < width and t.size(0) > 1):
+            raise ValueError(f"{name}: contiguous, separate rows expected, got shape {tuple(t.shape)} with strides {t.stride()}")
+        return ld if ld >= width else width
 
     def quantize_mxfp4_rows(self, x):
         """x bf16 / fp32 [M, K] (rows may be strided, any K) -> MXFP4Rows."""
@@ -848,7 +845,7 @@ class HipOps:
         else:
             # scratch for the quantised rows (PyTorch owns the memory); few whole-block rows are quantised inside the product
             ws, wsp, wsn, slabs = None, 0, 0, (K + 255) // 256
-            if M > 16 or K % 32 or ldx % 8 or x.data_ptr() % 16 or M * (slabs * 136 + 16) > 48 * 1024:
+            if M > 32 or K % 32 or ldx % 8 or x.data_ptr() % 16 or M * (slabs * 136 + 16) > 48 * 1024:
                 wsn = M * slabs * 128 + (M + 31) // 32 * slabs * 256            # fw_linear_mxfp4_workspace_bytes
                 ws = torch.empty(wsn, dtype=torch.uint8, device=xt.device)
                 wsp = ws.data_ptr()
@@ -890,21 +887,19 @@ class HipOps:
                 raise ValueError(f"y, x_out: x's shape {tuple(x.shape)} expected, got {tuple(y.shape)}, {tuple(x_out.shape)}")
             if not post:
                 post_w = None
-        groups, ptrs = 0, []
+        st = self._enter(x, y, x_out, bias, g1, g0, post_w, w, b, scale, shift, h_out)
+        groups = 0
         for name, v, many in (("bias", bias, False), ("g1", g1, True), ("g0", g0, True), ("post_w", post_w, False), ("w", w, False), ("b", b, False),
                               ("scale", scale, True), ("shift", shift, True)):
             if v is None:
-                ptrs.append(0)
                 continue
             n = v.numel() // C
-            if v.dtype is not torch.float32 or v.shape[-1:] != (C,) or not v.is_contiguous() or n < 1 or (n > 1 and not many):
+            if v.dtype is not torch.float32 or v.dim() < 1 or v.size(-1) != C or not v.is_contiguous() or n < 1 or (n > 1 and not many):
                 raise ValueError(f"{name}: contiguous fp32 [{C}]" + (f" or [groups, {C}]" if many else "") + f" expected, got {v.dtype} {tuple(v.shape)}")
             if many and n != groups:
                 if groups or rows % n:
                     raise ValueError(f"{name}: {n} vectors for {rows} rows; g1, g0, scale and shift alike in number, a divisor of the rows, expected")
                 groups = n
-            ptrs.append(v.data_ptr())
-        st = self._enter(x, y, x_out, bias, g1, g0, post_w, w, b, scale, shift, h_out)
         if out == "mxfp4":
             if h_out is not None:
                 raise ValueError("h_out takes bf16 rows: MXFP4 rows are allocated by the call")
@@ -920,7 +915,8 @@ class HipOps:
                     raise ValueError(f"h_out: x's shape {tuple(x.shape)} expected, got {tuple(h.shape)}")
             hp = h.data_ptr()
         _check(self.lib.fw_residual_norm(
-            x.data_ptr(), ldx, xop, ldxo, _dt(x), yp, ldy, ydt, ptrs[0], ptrs[1], ptrs[2], post, ptrs[3], RNORM[norm], ptrs[4], ptrs[5], ptrs[6], ptrs[7], eps,
+            x.data_ptr(), ldx, xop, ldxo, _dt(x), yp, ldy, ydt, _ptr(bias), _ptr(g1), _ptr(g0), post, _ptr(post_w), RNORM[norm], _ptr(w), _ptr(b),
+            _ptr(scale), _ptr(shift), eps,
             hp, ldh, hdt, hsp, rows, C, max(1, rows // (groups or 1)), st), "fw_residual_norm")
         return h
 

@@ -476,14 +476,15 @@ int fw_mxfp4_dequant_rows(const uint8_t* q, int64_t ldq, const uint8_t* s, void*
  * fw_gemm_bf16's epilogue (bias -> act -> per-column affine g1 / g0 -> + residual -> out_dtype).  C may alias res.
  * out_dtype FW_DT_MXFP4: the result is rounded to bf16 and quantised along N by the rule above -- the bytes of fw_mxfp4_quant_rows on the
  * bf16 output -- C = codes [M][ldc] (bytes), cs = scales; the input of the next MXFP4 linear without a pass of its own (cs is not used
- * for the other types).  lda, ldw (bytes) < 2^23. */
+ * for the other types).  lda, ldw (bytes) < 2^23.  A row's bits depend on nothing but the row -- except that products of up to 32 rows add
+ * their terms in another order than those of more. */
 int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, const uint8_t* W, int64_t ldw, const uint8_t* sw,
                   void* C, int64_t ldc, int out_dtype, uint8_t* cs, int M, int N, int K,
                   const float* bias, int act, const float* g1, const float* g0,
                   const void* res, int64_t ldr, int res_dtype, void* stream);
 
 /* The whole linear from bf16 rows: x [M][K] (ldx elements, any alignment of the element type) is quantised into the workspace and multiplied --
- * or, up to 16 rows with K % 32 == 0, 16-byte aligned rows and M (roundup(K, 256) 17 / 32 + 16) <= 48 KiB, quantised inside the product in one
+ * or, up to 32 rows with K % 32 == 0, 16-byte aligned rows and M (roundup(K, 256) 17 / 32 + 16) <= 48 KiB, quantised inside the product in one
  * launch, which reads no workspace (NULL, 0).  The rest as fw_gemm_mxfp4.  workspace: fw_linear_mxfp4_workspace_bytes(M, K) bytes, 16-byte
  * aligned, the caller's until the call's work is done on `stream`. */
 int64_t fw_linear_mxfp4_workspace_bytes(int M, int K);

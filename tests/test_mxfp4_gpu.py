@@ -302,3 +302,21 @@ def test_refusals(ops):
         ops.quantize_mxfp4_rows(x.cpu())
     with pytest.raises(KeyError):
         ops.linear(x, lin, act="tanh")
+
+
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 31, 32, 33])
+@pytest.mark.parametrize("N,K", [(40, 96), (1030, 2816), (4100, 288), (5000, 1440), (9000, 512)])
+def test_few_rows(ops, M, N, K):
+    """Every width of a work-group's columns (it follows N), one launch and two (rows behind an odd row stride), bf16 and MXFP4 output: one result."""
+    x, w, b = rnd(M, K, seed=1).cuda(), rnd(N, K, seed=2, scale=K ** -0.5), rnd(N, seed=3, scale=0.1, dtype=torch.float32)
+    wide = torch.zeros(M, K + 3, dtype=torch.bfloat16, device="cuda")
+    wide[:, :K] = x
+    lin, res = ops.pack_linear_mxfp4(w, b), rnd(M, N, seed=4).cuda()
+    want, err = product64(x, w, b, "gelu_erf", res=res)
+    got = ops.linear(x, lin, act="gelu_erf", res=res, out_f32=True)
+    close(got, want, err)
+    assert torch.equal(got, ops.linear(wide[:, :K], lin, act="gelu_erf", res=res, out_f32=True))
+    assert torch.equal(got, ops.linear(ops.quantize_mxfp4_rows(x), lin, act="gelu_erf", res=res, out_f32=True))
+    h, f = ops.linear(x, lin, act="gelu_erf"), ops.linear(x, lin, act="gelu_erf", out_mxfp4=True)
+    q = ops.quantize_mxfp4_rows(h)
+    assert torch.equal(q.q, f.q) and torch.equal(bytes_of(q), bytes_of(f))
