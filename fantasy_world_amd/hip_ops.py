@@ -864,8 +864,8 @@ class HipOps:
     def residual_norm(self, x, y=None, bias=None, g1=None, g0=None, post=None, post_w=None, w=None, b=None, scale=None, shift=None,
                       norm="layer", eps=1e-6, x_out=None, out="bf16", h_out=None):
         """x' = x + [post norm](y + bias) * g1 + g0, written to x_out (default: x, in place); -> h = norm(x') * w + b, * (1 + scale) + shift, as
-        bf16 rows (h_out: written there, rows may be strided) or (out="mxfp4") MXFP4Rows.  y None: h alone.  x, x_out [rows, C] fp32 or bf16, y fp32 or bf16; bias / post_w / w / b [C];
-        g1 / g0 / scale / shift [C], or all of them [groups, C] with rows % groups == 0: equal runs of rows share a vector.  post: None, "layer" or "rms"
+        bf16 rows (h_out: written there, rows may be strided) or (out="mxfp4") MXFP4Rows.  y None: h alone, and the update's arguments are not
+        looked at.  x, x_out [rows, C] fp32 or bf16, y fp32 or bf16; bias / post_w / w / b [C]; g1 / g0 / scale / shift [C], or all of them [groups, C] with rows % groups == 0: equal runs of rows share a vector.  post: None, "layer" or "rms"
         (post_w only with it); norm: "layer" or "rms" (b only with w)."""
         ldx = self._rows("x", x, torch.float32, torch.bfloat16)
         if out not in ("bf16", "mxfp4") or norm not in ("layer", "rms") or post not in RNORM:
