@@ -787,7 +787,7 @@ class HipOps:
     def pack_linear_mxfp4(self, w, b):
         """w [N, K] (any K) -> LinearMXFP4: the fp32 / bf16 weights quantised along K, the bias in fp32."""
         w = w.detach().to(device=self.device)
-        mx = self.quantize_mxfp4_rows(w if w.dtype == torch.bfloat16 else w.to(torch.float32))
+        mx = self.quantize_mxfp4_rows((w if w.dtype == torch.bfloat16 else w.to(torch.float32)).contiguous())
         return LinearMXFP4(mx.q, mx.s, None if b is None else self.to_f32(b), mx.K)
 
     def linear_from_mxfp4(self, q, s, b, K):
@@ -797,7 +797,8 @@ class HipOps:
         return lin
 
     def _linear_mxfp4(self, x, lin, act=None, g1=None, g0=None, res=None, out_f32=False, out=None, out_mxfp4=False):
-        """bf16 rows (quantised here) or MXFP4Rows x -> epilogue(x W^T): bf16, fp32 or MXFP4Rows."""
+        """bf16 rows (quantised here) or MXFP4Rows x -> epilogue(x W^T): bf16, fp32 or MXFP4Rows.  out may be res, but not x: work-groups read
+        all of x while others store."""
         N = lin.N
         ready = isinstance(x, MXFP4Rows)
         if ready:
@@ -835,6 +836,8 @@ class HipOps:
                 ldc, odt = self._rows("out", out, torch.bfloat16, torch.float32), _dt(out)
                 if out.shape != (M, N):
                     raise ValueError(f"out: [{M}, {N}] expected, got {tuple(out.shape)}")
+                if M and out.data_ptr() == (x.qp if ready else x.data_ptr()):
+                    raise ValueError("out must not be x")
             yp, csp = y.data_ptr(), 0
         tok = None if self._timing is None else self._time_begin(
             dict(kind="linear", M=M, N=N, K=K, res=res is not None, out_f32=odt == FW_DT_F32, act=act, mxfp4=True))
@@ -865,8 +868,9 @@ class HipOps:
                       norm="layer", eps=1e-6, x_out=None, out="bf16", h_out=None):
         """x' = x + [post norm](y + bias) * g1 + g0, written to x_out (default: x, in place); -> h = norm(x') * w + b, * (1 + scale) + shift, as
         bf16 rows (h_out: written there, rows may be strided) or (out="mxfp4") MXFP4Rows.  y None: h alone, and the update's arguments are not
-        looked at.  x, x_out [rows, C] fp32 or bf16, y fp32 or bf16; bias / post_w / w / b [C]; g1 / g0 / scale / shift [C], or all of them [groups, C] with rows % groups == 0: equal runs of rows share a vector.  post: None, "layer" or "rms"
-        (post_w only with it); norm: "layer" or "rms" (b only with w)."""
+        looked at.  x, x_out [rows, C] fp32 or bf16, y fp32 or bf16, C <= 8192; bias / post_w / w / b [C]; g1 / g0 / scale / shift [C], or all
+        of them [groups, C] with rows % groups == 0: equal runs of rows share a vector.  post: None, "layer" or "rms" (post_w only with it);
+        norm: "layer" or "rms" (b only with w)."""
         ldx = self._rows("x", x, torch.float32, torch.bfloat16)
         if out not in ("bf16", "mxfp4") or norm not in ("layer", "rms") or post not in RNORM:
             raise ValueError(f"out: 'bf16' | 'mxfp4', norm: 'layer' | 'rms', post: None | 'layer' | 'rms'; got {out!r}, {norm!r}, {post!r}")

@@ -320,3 +320,34 @@ def test_few_rows(ops, M, N, K):
     h, f = ops.linear(x, lin, act="gelu_erf"), ops.linear(x, lin, act="gelu_erf", out_mxfp4=True)
     q = ops.quantize_mxfp4_rows(h)
     assert torch.equal(q.q, f.q) and torch.equal(bytes_of(q), bytes_of(f))
+
+
+def test_rows_of_the_callers_own(ops):
+    """Codes that are a column slice of a wider buffer, as activations and as weights; a transposed weight view; what the kernels cannot read."""
+    M, N, K = 70, 96, 512
+    x, w, b = rnd(M, K, seed=1).cuda(), rnd(N, K, seed=2, scale=K ** -0.5).cuda(), rnd(N, seed=3, dtype=torch.float32).cuda()
+    mx, wm = ops.quantize_mxfp4_rows(x), ops.quantize_mxfp4_rows(w)
+    want = ops.linear(x, ops.pack_linear_mxfp4(w, b))
+    assert torch.equal(want, ops.linear(x, ops.pack_linear_mxfp4(w.t().contiguous().t(), b)))
+    from fantasy_world_amd.hip_ops import MXFP4Rows
+    wide = torch.full((N, 512), 0x77, dtype=torch.uint8, device="cuda")
+    for at in (0, 16, 256):
+        wq, xq = wide.clone(), torch.full((M, 544), 0x77, dtype=torch.uint8, device="cuda")
+        xq[:, at:at + 256], wq[:, at:at + 256] = mx.q, wm.q
+        lin = ops.linear_from_mxfp4(wq[:, at:at + 256], wm.s, b, K)
+        assert torch.equal(want, ops.linear(MXFP4Rows(xq[:, at:at + 256], mx.s, K), lin))
+        assert torch.equal(ops.dequantize_mxfp4_rows(MXFP4Rows(xq[:, at:at + 256], mx.s, K)), ops.dequantize_mxfp4_rows(mx))
+    odd = torch.zeros(M, 544, dtype=torch.uint8, device="cuda")
+    with pytest.raises(RuntimeError):
+        ops.linear(MXFP4Rows(odd[:, 8:264], mx.s, K), ops.pack_linear_mxfp4(w, b))
+    with pytest.raises(ValueError):
+        MXFP4Rows(odd[:, :250], mx.s, K)
+
+
+def test_the_output_is_not_the_input(ops):
+    lin, x = ops.pack_linear_mxfp4(rnd(256, 256, seed=1, scale=0.06), None), rnd(9, 256, seed=2).cuda()
+    with pytest.raises(ValueError):
+        ops.linear(x, lin, out=x)
+    want = ops.linear(x, lin, res=x)
+    buf = torch.empty_like(x)
+    assert torch.equal(ops.linear(x, lin, res=x, out=buf), want)

@@ -196,3 +196,44 @@ def test_refusals(ops):
         ops.residual_norm(x, y.cpu())
     with pytest.raises(RuntimeError):
         ops.residual_norm(rnd(2, 8193))
+
+
+@pytest.mark.parametrize("post", [None, "rms"])
+@pytest.mark.parametrize("rows,C,groups", [(4098, 1024, 3), (8194, 5120, 2), (4160, 256, 64), (4160, 512, 65)])
+def test_many_rows_in_groups(ops, rows, C, groups, post):
+    """Runs of rows with vectors of their own, from a run per work-group up to more runs than the kernel with staged vectors takes."""
+    x, y, v = rnd(rows, C, seed=1, scale=2.0), rnd(rows, C, seed=2, dtype=torch.bfloat16), vectors(C, groups, post=post)
+    check(ops, x.clone(), y, post=post, **v)
+    check(ops, x, y, post=post, out="mxfp4", x_out=torch.empty_like(x), **v)
+
+
+@pytest.mark.parametrize("rows,C", [(7, 5120), (4100, 5120), (4100, 640), (50, 333)])
+def test_captured_and_into_the_callers_rows(ops, rows, C):
+    """h in a column slice of the caller's, the rest of it untouched; a captured call replayed with eager work between: the eager bits."""
+    x, y, v = rnd(rows, C, seed=1), rnd(rows, C, seed=2, dtype=torch.bfloat16), vectors(C, post="layer")
+    xo = torch.empty_like(x)
+    want = ops.residual_norm(x, y, post="layer", x_out=xo, **v)
+    keep_x = xo.clone()
+    wide = torch.full((rows, C + 24), 5.0, dtype=torch.bfloat16, device="cuda")
+    for at in (0, 8, 3):
+        part = wide[:, at:at + C]
+        assert ops.residual_norm(x, y, post="layer", x_out=xo, h_out=part, **v) is part and torch.equal(part, want)
+        assert (wide[:, :at] == 5).all() and (wide[:, at + C:] == 5).all()
+        wide.fill_(5.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h = ops.residual_norm(x, y, post="layer", x_out=xo, **v)
+        q = ops.residual_norm(xo, None, out="mxfp4", w=v["w"], b=v["b"], scale=v["scale"], shift=v["shift"])
+    for _ in range(3):
+        xo.zero_()
+        h.zero_()
+        graph.replay()
+        again = ops.residual_norm(x, y, post="layer", x_out=torch.empty_like(x), **v)
+        torch.cuda.synchronize()
+        assert torch.equal(h, want) and torch.equal(xo, keep_x) and torch.equal(again, want)
+        assert torch.equal(q.q, ops.quantize_mxfp4_rows(want).q)
+    for bad in (wide[:, :C - 1], wide.float()[:, :C], wide[:rows - 1, :C]):
+        with pytest.raises(ValueError):
+            ops.residual_norm(x, y, h_out=bad, x_out=xo)
+    with pytest.raises(ValueError):
+        ops.residual_norm(x, y, h_out=wide[:, :C], x_out=xo, out="mxfp4")
