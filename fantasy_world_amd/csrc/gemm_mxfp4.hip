@@ -23,7 +23,7 @@ struct MxArgs {
     int M, N, slabs;
     const float* bias; int act; const float* g1; const float* g0;
     const void* res; int64_t ldr; int res_dtype;
-    int tiles_m, tiles_n, vec, cslabs;
+    int tiles_m, tiles_n, vec, cslabs, past;
 };
 
 // the upper half of the 8-register operand type is not read for fp4
@@ -84,21 +84,30 @@ __device__ __forceinline__ void mx_by_act(int act, F&& f) {
 // VEC: every row of C and of the residual is 16-byte accessible and N % 8 == 0; otherwise (and RES < 0) element by element.
 // With a residual and no activation all of a quadrant's residual rows are in flight before the transpose and the next quadrant's are issued
 // as registers free up; with an activation as well (ACT_TOO) they follow the transpose, in the registers that the accumulators leave.
-template <int RES, bool VEC, bool ACT_TOO, int RBK, int NQ, typename Acc>
+// HALVES (fp32 residual and fp32 output): a lane's 8 columns are 4 + 4, one half of the 64 each, so that the 8 lanes of a row touch 128
+// contiguous bytes in every access; 8 consecutive fp32 are two accesses that each touch all 256 bytes.  Which half is first alternates
+// with the row: the LDS reads then stay free of conflicts.  32760 x 5120 x 5120 with gate and residual in place:
+// 566 us, 594 with 8 consecutive ones.
+template <int RES, bool VEC, bool ACT_TOO, bool HALVES, bool PAST, int RBK, int NQ, typename Acc>
 __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Acc& acc, int lane, int m0, int n0) {
     const int fi = lane & 31, hi = lane >> 5, q = lane & 7, rl = lane >> 3;
-    const int col = n0 + q * 8;
-    const bool in = col < p.N;
+    // this lane's columns: col .. + 3 and col2 .. + 3
+    const int lc = HALVES ? 32 * (rl & 1) + q * 4 : q * 8, lc2 = HALVES ? lc ^ 32 : lc + 4;
+    const int col = n0 + lc, col2 = n0 + lc2;
+    const bool in = col < p.N, in2 = HALVES ? col2 < p.N : in;
+    // and where they lie in a row of the LDS image
+    const int at_lo = HALVES ? (lc >> 3) * 16 + ((q ^ rl) & 1) * 128 : q * 16 + (rl & 1) * 128;
+    const int at_up = HALVES ? (lc2 >> 3) * 16 + ((q ^ rl) & 1) * 128 : q * 16 + ((rl & 1) ^ 1) * 128;
     const int res_dtype = RES < 0 ? p.res_dtype : RES;
     constexpr int IT = 4 * RBK;                           // steps of 8 rows
     u32x4_t rv[IT][RES == FW_DT_F32 ? 2 : 1];
     auto load_res = [&](int it, int row0) __attribute__((always_inline)) {
         const int row = row0 + rl;
-        if (VEC && RES > 0 && in && row < p.M) {
+        if (VEC && RES > 0 && (HALVES || in) && row < p.M) {
             // a scalar row address and a 32-bit lane offset: 64-bit addresses of 16 loads do not fit next to the accumulators
-            const char* r = (const char*)p.res + ((int64_t)row0 * p.ldr + n0) * (RES == FW_DT_F32 ? 4 : 2) + (unsigned)(rl * (int)p.ldr + q * 8) * (RES == FW_DT_F32 ? 4u : 2u);
-            rv[it][0] = *(const u32x4_t*)r;
-            if (RES == FW_DT_F32) rv[it][RES == FW_DT_F32 ? 1 : 0] = *(const u32x4_t*)(r + 16);
+            const char* r = (const char*)p.res + ((int64_t)row0 * p.ldr + n0) * (RES == FW_DT_F32 ? 4 : 2) + (unsigned)(rl * (int)p.ldr + lc) * (RES == FW_DT_F32 ? 4u : 2u);
+            if (!HALVES || in) rv[it][0] = fw_load<PAST, u32x4_t>(r);
+            if (RES == FW_DT_F32 && (!HALVES || in2)) rv[it][RES == FW_DT_F32 ? 1 : 0] = fw_load<PAST, u32x4_t>(r + (lc2 - lc) * 4);
         }
     };
     if (VEC && RES > 0 && !ACT_TOO) {
@@ -111,8 +120,9 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
     for (int j = 0; j < 2; ++j) bias[j] = p.bias && n0 + j * 32 + fi < p.N ? p.bias[n0 + j * 32 + fi] : 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        g1[j] = p.g1 && col + j < p.N ? p.g1[col + j] : 1.f;
-        g0[j] = p.g0 && col + j < p.N ? p.g0[col + j] : 0.f;
+        const int c = j < 4 ? col + j : col2 + j - 4;
+        g1[j] = p.g1 && c < p.N ? p.g1[c] : 1.f;
+        g0[j] = p.g0 && c < p.N ? p.g0[c] : 0.f;
     }
     auto quadrant = [&](auto q_tag) __attribute__((always_inline)) {
         constexpr int Q = decltype(q_tag)::value;
@@ -138,7 +148,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
             const int row_l = it * 8 + rl, row = m0 + Q * 32 * RBK + row_l;
-            const f32x4_t lo = *(const f32x4_t*)(reg + row_l * 256 + q * 16 + (rl & 1) * 128), up = *(const f32x4_t*)(reg + row_l * 256 + q * 16 + ((rl & 1) ^ 1) * 128);
+            const f32x4_t lo = *(const f32x4_t*)(reg + row_l * 256 + at_lo), up = *(const f32x4_t*)(reg + row_l * 256 + at_up);
             float v[8] = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
             if (affine) {
 #pragma unroll
@@ -159,7 +169,11 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
                     if (col + j < p.N) v[j] += res_dtype == FW_DT_F32 ? ((const float*)p.res)[o] : bf16_bits_to_f32(((const uint16_t*)p.res)[o]);
                 }
             }
-            if (p.out_dtype == FW_DT_MXFP4) {
+            if (HALVES) {
+                const int64_t o = (int64_t)row * p.ldc;
+                if (live && in) fw_store<PAST>((float*)p.C + o + col, f32x4_t{v[0], v[1], v[2], v[3]});
+                if (live && in2) fw_store<PAST>((float*)p.C + o + col2, f32x4_t{v[4], v[5], v[6], v[7]});
+            } else if (p.out_dtype == FW_DT_MXFP4) {
                 // the value is rounded to bf16 first: a fused quantisation returns the bytes of fw_mxfp4_quant_rows on the bf16 output.
                 // Columns past N are zeros of the padded row (the launcher's grid covers all of it).
                 u32x4_t h;
@@ -182,7 +196,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
                         *(f32x4_t*)((float*)p.C + o) = f32x4_t{v[0], v[1], v[2], v[3]};
                         *(f32x4_t*)((float*)p.C + o + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
                     } else {
-                        *(u32x4_t*)((uint16_t*)p.C + o) = u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+                        fw_store<PAST>((uint16_t*)p.C + o, u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])});
                     }
                 } else {
 #pragma unroll
@@ -199,16 +213,27 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& p, char* reg, const Ac
     if constexpr (NQ > 1) quadrant(std::integral_constant<int, 1>{});
 }
 
-template <int RBK, int NQ, typename Acc>
+// BIG: with outputs larger than the memory-side cache (256 MB; p.past), which are stored past the caches, the residual read the same way: they
+// would only push the operands out (32760 x 5120 x 5120 with gate and fp32 residual: 573 us, 507 so; with the norm that reads it 758 and
+// 702).  A smaller output stays where its reader finds it (8190 rows: 139 us, 156 past the caches).
+template <bool BIG, int RBK, int NQ, typename Acc>
 __device__ __forceinline__ void mx_finish(const MxArgs& p, char* reg, const Acc& acc, int lane, int m0, int n0) {
     const bool act = p.act != FW_ACT_NONE;
-    if (!p.vec) mx_epilogue<-1, false, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
-    else if (p.res_dtype == FW_DT_NONE) mx_epilogue<FW_DT_NONE, true, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
+    if constexpr (BIG) {
+        if (p.past && p.vec) {
+            if (p.res_dtype == FW_DT_NONE) { mx_epilogue<FW_DT_NONE, true, true, false, true, RBK, NQ>(p, reg, acc, lane, m0, n0); return; }
+            if (p.res_dtype == FW_DT_F32 && p.out_dtype == FW_DT_F32 && !act) { mx_epilogue<FW_DT_F32, true, false, true, true, RBK, NQ>(p, reg, acc, lane, m0, n0); return; }
+            if (p.res_dtype == FW_DT_BF16 && !act) { mx_epilogue<FW_DT_BF16, true, false, false, true, RBK, NQ>(p, reg, acc, lane, m0, n0); return; }
+        }
+    }
+    if (!p.vec) mx_epilogue<-1, false, true, false, false, RBK, NQ>(p, reg, acc, lane, m0, n0);
+    else if (p.res_dtype == FW_DT_NONE) mx_epilogue<FW_DT_NONE, true, true, false, false, RBK, NQ>(p, reg, acc, lane, m0, n0);
     else if (p.res_dtype == FW_DT_F32) {
-        if (act) mx_epilogue<FW_DT_F32, true, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
-        else mx_epilogue<FW_DT_F32, true, false, RBK, NQ>(p, reg, acc, lane, m0, n0);
-    } else if (act) mx_epilogue<FW_DT_BF16, true, true, RBK, NQ>(p, reg, acc, lane, m0, n0);
-    else mx_epilogue<FW_DT_BF16, true, false, RBK, NQ>(p, reg, acc, lane, m0, n0);
+        if (act) mx_epilogue<FW_DT_F32, true, true, false, false, RBK, NQ>(p, reg, acc, lane, m0, n0);
+        else if (p.out_dtype == FW_DT_F32) mx_epilogue<FW_DT_F32, true, false, true, false, RBK, NQ>(p, reg, acc, lane, m0, n0);
+        else mx_epilogue<FW_DT_F32, true, false, false, false, RBK, NQ>(p, reg, acc, lane, m0, n0);
+    } else if (act) mx_epilogue<FW_DT_BF16, true, true, false, false, RBK, NQ>(p, reg, acc, lane, m0, n0);
+    else mx_epilogue<FW_DT_BF16, true, false, false, false, RBK, NQ>(p, reg, acc, lane, m0, n0);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -310,7 +335,7 @@ __global__ __launch_bounds__(512, ST * (BM + BN) * 136 <= 80 * 1024 ? 4 : 2) voi
         cur = cur + 1 == ST ? 0 : cur + 1;
     }
     FWX_BARRIER();                                        // everybody has read the last slab: the stages become the epilogue's space
-    mx_finish<(WM < 2 ? 1 : 2), (WM < 2 ? 1 : WM / 2)>(p, smem + wave * 16384, acc, lane, m0 + wm * WM * 32, n0 + wn * 64);
+    mx_finish<false, (WM < 2 ? 1 : 2), (WM < 2 ? 1 : WM / 2)>(p, smem + wave * 16384, acc, lane, m0 + wm * WM * 32, n0 + wn * 64);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -466,7 +491,7 @@ __global__ __launch_bounds__(512, 2) void gemm_mxfp4_256_kernel(MxArgs p) {
     };
     if (grp == 0) { mainloop(std::integral_constant<int, 0>{}); FWX_BARRIER(); }
     else mainloop(std::integral_constant<int, 1>{});
-    mx_finish<2, 2>(p, smem + wave * 16384, acc, lane, m0 + grp * 128, n0 + wn * 64);
+    mx_finish<true, 2, 2>(p, smem + wave * 16384, acc, lane, m0 + grp * 128, n0 + wn * 64);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -685,6 +710,7 @@ static int mx_args(MxArgs& p, const uint8_t* W, int64_t ldw, const uint8_t* sw, 
     const int ce = out_dtype == FW_DT_F32 ? 4 : 8, re = res_dtype == FW_DT_F32 ? 4 : 8;
     p.vec = (N % 8) == 0 && (out_dtype == FW_DT_MXFP4 || ((ldc % ce) == 0 && (((uintptr_t)C) & 15) == 0)) &&
             (res_dtype == FW_DT_NONE || ((ldr % re) == 0 && (((uintptr_t)res) & 15) == 0 && ldr < (1 << 26)));
+    p.past = out_dtype != FW_DT_MXFP4 && (int64_t)M * N * (out_dtype == FW_DT_F32 ? 4 : 2) > FW_CACHE_BYTES;
     return 0;
 }
 

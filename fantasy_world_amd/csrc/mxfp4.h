@@ -59,3 +59,17 @@ __device__ __forceinline__ uint32_t mx_pack8_f32(const float* f, float scale) {
     r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[4], f[5], scale, 2);
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[6], f[7], scale, 3);
 }
+
+// An array larger than the memory-side cache gains nothing from passing through the caches and costs what else lies there: PAST accesses go
+// past them.
+constexpr int64_t FW_CACHE_BYTES = (int64_t)256 << 20;
+template <bool PAST, typename V>
+__device__ __forceinline__ V fw_load(const void* a) {
+    if constexpr (PAST) return __builtin_nontemporal_load((const V*)a);
+    else return *(const V*)a;
+}
+template <bool PAST, typename V>
+__device__ __forceinline__ void fw_store(void* a, V v) {
+    if constexpr (PAST) __builtin_nontemporal_store(v, (V*)a);
+    else *(V*)a = v;
+}

@@ -24,7 +24,10 @@ struct RnArgs {
 // or has not (a type, a vector) is one uniform branch a group.
 constexpr int rn_group(int vpl) { return vpl < 4 ? vpl : 4; }
 
-template <int MODE, int G>
+// PAST: a stream larger than the memory-side cache (256 MB) is read and written past the caches -- what a row leaves there is gone before
+// anybody comes back for it, and it costs the rows that follow.  32760 x 5120 in place, fp32 stream, bf16 y: bf16 h 397 us, 376 so; MXFP4 h
+// 364 and 308.  A smaller stream finds part of itself there (8190 x 5120: 90 us, 95 past the caches).
+template <int MODE, bool PAST, int G>
 __device__ __forceinline__ void rn_load(const char* row, bool f32, int lane, int i0, int C, f32x4_t (&t)[G]) {
 #pragma unroll
     for (int i = 0; i < G; ++i) t[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -32,7 +35,7 @@ __device__ __forceinline__ void rn_load(const char* row, bool f32, int lane, int
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             const int c = (lane + 64 * (i0 + i)) * 4;
-            if (MODE == 2 || (MODE == 1 && c < C)) t[i] = *(const f32x4_t*)(row + lane * 16 + (i0 + i) * 1024);
+            if (MODE == 2 || (MODE == 1 && c < C)) t[i] = fw_load<PAST, f32x4_t>(row + lane * 16 + (i0 + i) * 1024);
             else if (MODE == 0) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) if (c + j < C) t[i][j] = ((const float*)row)[c + j];
@@ -43,7 +46,7 @@ __device__ __forceinline__ void rn_load(const char* row, bool f32, int lane, int
         for (int i = 0; i < G; ++i) {
             const int c = (lane + 64 * (i0 + i)) * 4;
             if (MODE == 2 || (MODE == 1 && c < C)) {
-                const u32x2_t r = *(const u32x2_t*)(row + lane * 8 + (i0 + i) * 512);
+                const u32x2_t r = fw_load<PAST, u32x2_t>(row + lane * 8 + (i0 + i) * 512);
                 t[i] = f32x4_t{__uint_as_float(r[0] << 16), __uint_as_float(r[0] & 0xffff0000u), __uint_as_float(r[1] << 16), __uint_as_float(r[1] & 0xffff0000u)};
             } else if (MODE == 0) {
 #pragma unroll
@@ -53,10 +56,10 @@ __device__ __forceinline__ void rn_load(const char* row, bool f32, int lane, int
     }
 }
 // 4 bf16 (two dwords) of chunk i
-template <int MODE>
+template <int MODE, bool PAST>
 __device__ __forceinline__ void rn_store_bf16(char* row, int lane, int i, int C, u32x2_t r) {
     const int c = (lane + 64 * i) * 4;
-    if (MODE == 2 || (MODE == 1 && c < C)) *(u32x2_t*)(row + lane * 8 + i * 512) = r;
+    if (MODE == 2 || (MODE == 1 && c < C)) fw_store<PAST>(row + lane * 8 + i * 512, r);
     else if (MODE == 0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) if (c + j < C) ((uint16_t*)row)[c + j] = (uint16_t)(r[j >> 1] >> (16 * (j & 1)));
@@ -111,14 +114,14 @@ struct RnParams {
 #pragma unroll
             for (int i = 0; i < G; ++i) t[i] = sm[slot * VPL * 64 + 64 * (i0 + i) + lane];
         } else {
-            rn_load<MODE, G>((const char*)(v + (k >= RN_G1 ? mo : 0)), true, lane, i0, MODE == 2 ? VPL * 256 : p.C, t);
+            rn_load<MODE, false, G>((const char*)(v + (k >= RN_G1 ? mo : 0)), true, lane, i0, MODE == 2 ? VPL * 256 : p.C, t);
         }
         return true;
     }
 };
 
 // x' of a group from x (v) and the finished y term (t): stored, and left in v as the norm reads it
-template <int VPL, int MODE, bool STAGE, int G>
+template <int VPL, int MODE, bool STAGE, bool PAST, int G>
 __device__ __forceinline__ void rn_update(const RnArgs& p, const RnParams<VPL, MODE, STAGE>& par, f32x4_t* v, f32x4_t (&t)[G], int i0, char* xo, bool xf) {
     const int lane = par.lane, C = MODE == 2 ? VPL * 256 : p.C;
     f32x4_t a[G], o[G];
@@ -141,7 +144,7 @@ __device__ __forceinline__ void rn_update(const RnArgs& p, const RnParams<VPL, M
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             const int c = (lane + 64 * (i0 + i)) * 4;
-            if (MODE == 2 || (MODE == 1 && c < C)) *(f32x4_t*)(xo + lane * 16 + (i0 + i) * 1024) = v[i];
+            if (MODE == 2 || (MODE == 1 && c < C)) fw_store<PAST>(xo + lane * 16 + (i0 + i) * 1024, v[i]);
             else if (MODE == 0) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) if (c + j < C) ((float*)xo)[c + j] = v[i][j];
@@ -151,7 +154,7 @@ __device__ __forceinline__ void rn_update(const RnArgs& p, const RnParams<VPL, M
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             const u32x2_t r = {pack_bf16x2(v[i][0], v[i][1]), pack_bf16x2(v[i][2], v[i][3])};
-            rn_store_bf16<MODE>(xo, lane, i0 + i, C, r);
+            rn_store_bf16<MODE, PAST>(xo, lane, i0 + i, C, r);
             v[i] = f32x4_t{__uint_as_float(r[0] << 16), __uint_as_float(r[0] & 0xffff0000u), __uint_as_float(r[1] << 16), __uint_as_float(r[1] & 0xffff0000u)};
         }
     }
@@ -164,7 +167,7 @@ __device__ __forceinline__ int64_t rn_uniform(int64_t off) {
     return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
 }
 
-template <int VPL, int MODE, bool POST, bool STAGE>
+template <int VPL, int MODE, bool POST, bool STAGE, bool PAST>
 __device__ __forceinline__ void rn_row(const RnArgs& p, const RnParams<VPL, MODE, STAGE>& par, int row) {
     constexpr int G = rn_group(VPL);
     const int C = MODE == 2 ? VPL * 256 : p.C, lane = par.lane;
@@ -174,12 +177,12 @@ __device__ __forceinline__ void rn_row(const RnArgs& p, const RnParams<VPL, MODE
     char* xo = (char*)p.xo + rn_uniform((int64_t)row * p.ldxo * (xf ? 4 : 2));
     f32x4_t v[VPL];
 #pragma unroll
-    for (int i0 = 0; i0 < VPL; i0 += G) rn_load<MODE, G>(xr, xf, lane, i0, C, *(f32x4_t(*)[G])(v + i0));
+    for (int i0 = 0; i0 < VPL; i0 += G) rn_load<MODE, PAST, G>(xr, xf, lane, i0, C, *(f32x4_t(*)[G])(v + i0));
     float mean, rstd;
     if (POST) {                                           // the statistics need all of y + bias
         f32x4_t t[VPL];
 #pragma unroll
-        for (int i0 = 0; i0 < VPL; i0 += G) rn_load<MODE, G>(yr, yf, lane, i0, C, *(f32x4_t(*)[G])(t + i0));
+        for (int i0 = 0; i0 < VPL; i0 += G) rn_load<MODE, PAST, G>(yr, yf, lane, i0, C, *(f32x4_t(*)[G])(t + i0));
 #pragma unroll
         for (int i0 = 0; i0 < VPL; i0 += G) {
             f32x4_t u[G];
@@ -198,21 +201,21 @@ __device__ __forceinline__ void rn_row(const RnArgs& p, const RnParams<VPL, MODE
 #pragma unroll
                 for (int i = 0; i < G; ++i) u[i] *= w[i];
             }
-            rn_update<VPL, MODE, STAGE, G>(p, par, v + i0, u, i0, xo, xf);
+            rn_update<VPL, MODE, STAGE, PAST, G>(p, par, v + i0, u, i0, xo, xf);
         }
     } else if (p.y) {                                     // a group of y at a time, the next one on its way: the row of x is all that stays
         f32x4_t t[2][G];
-        rn_load<MODE, G>(yr, yf, lane, 0, C, t[0]);
+        rn_load<MODE, PAST, G>(yr, yf, lane, 0, C, t[0]);
 #pragma unroll
         for (int i0 = 0; i0 < VPL; i0 += G) {
             f32x4_t (&u)[G] = t[(i0 / G) & 1];
-            if (i0 + G < VPL) rn_load<MODE, G>(yr, yf, lane, i0 + G, C, t[(i0 / G + 1) & 1]);
+            if (i0 + G < VPL) rn_load<MODE, PAST, G>(yr, yf, lane, i0 + G, C, t[(i0 / G + 1) & 1]);
             f32x4_t b[G];
             if (par.get(RN_BIAS, i0, b)) {
 #pragma unroll
                 for (int i = 0; i < G; ++i) u[i] += b[i];
             }
-            rn_update<VPL, MODE, STAGE, G>(p, par, v + i0, u, i0, xo, xf);
+            rn_update<VPL, MODE, STAGE, PAST, G>(p, par, v + i0, u, i0, xo, xf);
         }
     }
     rn_stats<VPL>(v, lane, C, p.norm == FW_RNORM_LAYER, p.eps, mean, rstd);
@@ -276,7 +279,7 @@ __device__ __forceinline__ void rn_row(const RnArgs& p, const RnParams<VPL, MODE
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < G; ++i) rn_store_bf16<MODE>(hr, lane, i0 + i, C, r[i]);
+            for (int i = 0; i < G; ++i) rn_store_bf16<MODE, PAST>(hr, lane, i0 + i, C, r[i]);
         }
     }
 }
@@ -287,14 +290,14 @@ __global__ __launch_bounds__(256) void residual_norm_kernel(RnArgs p) {
     const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));      // uniform: addresses in scalar registers
     if (row >= p.rows) return;
     const RnParams<VPL, MODE, false> par{p, nullptr, (int)threadIdx.x & 63, (int64_t)(row / p.rows_per_mod) * p.C};
-    rn_row<VPL, MODE, POST, false>(p, par, row);
+    rn_row<VPL, MODE, POST, false, false>(p, par, row);
 }
 
 // Many rows: a work-group stages the parameter vectors of one run of rows in LDS and walks that run with the run's other work-groups.
 // Through the caches the vectors cost more than the row itself (bias, g1, scale, shift: 80 KiB per 60 KiB row at C = 5120): 32760 x 5120
 // takes 923 us that way.  The work-groups walk side by side: with a contiguous block of rows for each, their equal strides of 2^18 bytes
 // and more fall on the same memory channels (522 us).
-template <int VPL, int MODE, bool POST>
+template <int VPL, int MODE, bool POST, bool PAST>
 __global__ __launch_bounds__(POST ? 256 : 512, POST ? 1 : 2) void residual_norm_staged_kernel(RnArgs p, int wgs_per_run) {
     extern __shared__ f32x4_t rn_smem[];
     constexpr int T = POST ? 256 : 512;
@@ -315,7 +318,7 @@ __global__ __launch_bounds__(POST ? 256 : 512, POST ? 1 : 2) void residual_norm_
         // the vectors stay in LDS: as invariants of this loop the compiler keeps them in 320 registers and spills
         int z = 0;
         asm volatile("" : "+s"(z));
-        rn_row<VPL, MODE, POST, true>(p, RnParams<VPL, MODE, true>{p, rn_smem + z, lane, 0}, __builtin_amdgcn_readfirstlane((int)r));
+        rn_row<VPL, MODE, POST, true, PAST>(p, RnParams<VPL, MODE, true>{p, rn_smem + z, lane, 0}, __builtin_amdgcn_readfirstlane((int)r));
     }
 }
 
@@ -332,7 +335,8 @@ int rn_launch(const RnArgs& p, hipStream_t st) {
             constexpr int waves = POST ? 4 : 8;
             const int per_cu = POST ? (lds <= 40 * 1024 ? 4 : lds <= 80 * 1024 ? 2 : 1) : (lds <= 80 * 1024 ? 2 : 1);
             const int wgs_per_run = min(256 * per_cu / runs, (min(p.rows, p.rows_per_mod) + waves - 1) / waves);
-            const auto f = residual_norm_staged_kernel<VPL, MODE, POST>;
+            const bool past = MODE == 2 && (int64_t)p.rows * p.C * (p.x_dtype == FW_DT_F32 ? 4 : 2) > FW_CACHE_BYTES;
+            const auto f = past ? residual_norm_staged_kernel<VPL, MODE, POST, MODE == 2> : residual_norm_staged_kernel<VPL, MODE, POST, false>;
             if (lds > 64 * 1024) {
                 const int rc = (int)hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
                 if (rc) return rc;

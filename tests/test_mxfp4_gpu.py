@@ -351,3 +351,30 @@ def test_the_output_is_not_the_input(ops):
     want = ops.linear(x, lin, res=x)
     buf = torch.empty_like(x)
     assert torch.equal(ops.linear(x, lin, res=x, out=buf), want)
+
+
+def test_arrays_larger_than_the_caches(ops):
+    """Outputs, residuals and rows of more than 256 MB are accessed past the caches: the bits of the same rows in smaller calls."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    M, N, K = 13200, 10304, 1024
+    x = torch.randn(M, K, generator=g, device="cuda").bfloat16()
+    lin, gate = ops.pack_linear_mxfp4(rnd(N, K, seed=2, scale=K ** -0.5), rnd(N, seed=3)), rnd(N, seed=4, dtype=torch.float32).cuda()
+    part = 2048                                           # enough rows for the same tiles, 84 MB of fp32 output
+    for rdt, kw in ((None, dict()), (None, dict(act="gelu_tanh")), (None, dict(out_f32=True)), (torch.bfloat16, dict(g1=gate)), (torch.bfloat16, dict(out_f32=True)),
+                    (torch.float32, dict(g1=gate, out_f32=True)), (torch.float32, dict()), (torch.float32, dict(act="silu", out_f32=True))):
+        res = None if rdt is None else torch.randn(M, N, generator=g, device="cuda").to(rdt)
+        got = ops.linear(x, lin, res=res, **kw)
+        for a in (0, 5 * part, M - part):
+            assert torch.equal(got[a:a + part], ops.linear(x[a:a + part], lin, res=None if res is None else res[a:a + part], **kw)), (rdt, kw)
+        if rdt is not None and got.dtype == rdt:          # in place
+            assert ops.linear(x, lin, res=res, out=res, **kw) is res and torch.equal(res, got)
+        del res, got
+    for dt in (torch.bfloat16, torch.float32):
+        rows = torch.randn(M, N, generator=g, device="cuda").to(dt)
+        mx = ops.quantize_mxfp4_rows(rows)
+        for a in (0, 4096, 12800):
+            assert torch.equal(mx.q[a:a + 400], ops.quantize_mxfp4_rows(rows[a:a + 400]).q)
+        back = ops.dequantize_mxfp4_rows(mx, dt)
+        check_rows(ops.quantize_mxfp4_rows(rows[12800:12864]), rows[12800:12864].cpu(), ops)
+        assert torch.equal(back[12800:12864], ops.dequantize_mxfp4_rows(ops.quantize_mxfp4_rows(rows[12800:12864]), dt))
+        assert torch.equal(back, ops.dequantize_mxfp4_rows(ops.quantize_mxfp4_rows(back), dt))       # values of the format are kept

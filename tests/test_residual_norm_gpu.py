@@ -237,3 +237,23 @@ def test_captured_and_into_the_callers_rows(ops, rows, C):
             ops.residual_norm(x, y, h_out=bad, x_out=xo)
     with pytest.raises(ValueError):
         ops.residual_norm(x, y, h_out=wide[:, :C], x_out=xo, out="mxfp4")
+
+
+@pytest.mark.parametrize("post", [None, "layer"])
+@pytest.mark.parametrize("xdt", [torch.float32, torch.bfloat16])
+def test_streams_larger_than_the_caches(ops, xdt, post):
+    """A stream of more than 256 MB is accessed past the caches: the bits of the same rows in smaller calls."""
+    rows, C = (13200, 5120) if xdt == torch.float32 else (26400, 5120)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, y = torch.randn(rows, C, generator=g, device="cuda").to(xdt), torch.randn(rows, C, generator=g, device="cuda").bfloat16()
+    v = vectors(C, post=post)
+    xo = torch.empty_like(x)
+    h = ops.residual_norm(x, y, post=post, x_out=xo, **v)
+    q = ops.residual_norm(x, y, post=post, x_out=torch.empty_like(x), out="mxfp4", **v)
+    for a in (0, 6000, rows - 5000):
+        part = x[a:a + 5000].clone()
+        want = ops.residual_norm(part, y[a:a + 5000], post=post, **v)
+        assert torch.equal(h[a:a + 5000], want) and torch.equal(xo[a:a + 5000], part)
+        assert torch.equal(q.q[a:a + 5000], ops.quantize_mxfp4_rows(want).q)
+    src = x.clone()
+    assert torch.equal(ops.residual_norm(x, y, post=post, **v), h) and torch.equal(x, xo) and not torch.equal(x, src)
