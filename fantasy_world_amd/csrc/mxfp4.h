@@ -73,3 +73,8 @@ __device__ __forceinline__ void fw_store(void* a, V v) {
     if constexpr (PAST) __builtin_nontemporal_store(v, (V*)a);
     else *(V*)a = v;
 }
+
+// Vectors at any alignment of their element (the hardware takes them so): rows of an odd length or from an odd column on.
+typedef f32x4_t __attribute__((aligned(4))) f32x4_odd_t;
+typedef u32x2_t __attribute__((aligned(2))) u32x2_odd_t;
+typedef u32x4_t __attribute__((aligned(2))) u32x4_odd_t;

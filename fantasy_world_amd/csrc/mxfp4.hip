@@ -12,12 +12,17 @@ __device__ __forceinline__ void load8(const void* x, int64_t off, int k, int K, 
         if (VEC) {
             const f32x4_t a = fw_load<PAST, f32x4_t>((const float*)x + off), b = fw_load<PAST, f32x4_t>((const float*)x + off + 4);
             f[0] = a[0]; f[1] = a[1]; f[2] = a[2]; f[3] = a[3]; f[4] = b[0]; f[5] = b[1]; f[6] = b[2]; f[7] = b[3];
+        } else if (k + 8 <= K) {
+            const f32x4_t a = *(const f32x4_odd_t*)((const float*)x + off), b = *(const f32x4_odd_t*)((const float*)x + off + 4);
+            f[0] = a[0]; f[1] = a[1]; f[2] = a[2]; f[3] = a[3]; f[4] = b[0]; f[5] = b[1]; f[6] = b[2]; f[7] = b[3];
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] = k + j < K ? ((const float*)x)[off + j] : 0.f;
         }
     } else if (VEC) {
         raw = fw_load<PAST, u32x4_t>((const uint16_t*)x + off);
+    } else if (k + 8 <= K) {
+        raw = *(const u32x4_odd_t*)((const uint16_t*)x + off);
     } else {
         uint32_t h[8];
 #pragma unroll
@@ -94,6 +99,9 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_rows_kernel(const uint8_t* 
             if (VEC) {
                 fw_store<PAST>((float*)y + off, f32x4_t{f[0], f[1], f[2], f[3]});
                 fw_store<PAST>((float*)y + off + 4, f32x4_t{f[4], f[5], f[6], f[7]});
+            } else if (k + 8 <= K) {
+                *(f32x4_odd_t*)((float*)y + off) = f32x4_t{f[0], f[1], f[2], f[3]};
+                *(f32x4_odd_t*)((float*)y + off + 4) = f32x4_t{f[4], f[5], f[6], f[7]};
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) if (k + j < K) ((float*)y)[off + j] = f[j];
@@ -101,6 +109,8 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_rows_kernel(const uint8_t* 
         } else {
             if (VEC) {
                 fw_store<PAST>((uint16_t*)y + off, u32x4_t{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])});
+            } else if (k + 8 <= K) {
+                *(u32x4_odd_t*)((uint16_t*)y + off) = u32x4_t{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) if (k + j < K) ((uint16_t*)y)[off + j] = f32_to_bf16_bits(f[j]);

@@ -18,7 +18,7 @@ struct RnArgs {
     int rows, C, rows_per_mod;
 };
 
-// MODE of a row access: 0 one value at a time (any C, any alignment), 1 four at a time (C % 4 == 0), 2 four at a time and C = 256 VPL, known at
+// MODE of a row access: 0 four at a time at any alignment, the row's last ones singly (any C), 1 four at a time, aligned (C % 4 == 0), 2 four at a time and C = 256 VPL, known at
 // compile time (no lane is ever past the row: per-chunk predicates cost registers and branches).
 // Chunk i of a row: lane l holds elements 4 l .. 4 l + 3 of its 256.  Everything below works on groups of G chunks, so that what a call has
 // or has not (a type, a vector) is one uniform branch a group.
@@ -36,21 +36,24 @@ __device__ __forceinline__ void rn_load(const char* row, bool f32, int lane, int
         for (int i = 0; i < G; ++i) {
             const int c = (lane + 64 * (i0 + i)) * 4;
             if (MODE == 2 || (MODE == 1 && c < C)) t[i] = fw_load<PAST, f32x4_t>(row + lane * 16 + (i0 + i) * 1024);
+            else if (MODE == 0 && c + 4 <= C) t[i] = *(const f32x4_odd_t*)(row + lane * 16 + (i0 + i) * 1024);
             else if (MODE == 0) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) if (c + j < C) t[i][j] = ((const float*)row)[c + j];
+                for (int j = 0; j < 3; ++j) if (c + j < C) t[i][j] = ((const float*)row)[c + j];
             }
         }
     } else {
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             const int c = (lane + 64 * (i0 + i)) * 4;
-            if (MODE == 2 || (MODE == 1 && c < C)) {
-                const u32x2_t r = fw_load<PAST, u32x2_t>(row + lane * 8 + (i0 + i) * 512);
+            if (MODE == 2 || (MODE == 1 ? c < C : c + 4 <= C)) {
+                u32x2_t r;
+                if constexpr (MODE == 0) r = *(const u32x2_odd_t*)(row + lane * 8 + (i0 + i) * 512);
+                else r = fw_load<PAST, u32x2_t>(row + lane * 8 + (i0 + i) * 512);
                 t[i] = f32x4_t{__uint_as_float(r[0] << 16), __uint_as_float(r[0] & 0xffff0000u), __uint_as_float(r[1] << 16), __uint_as_float(r[1] & 0xffff0000u)};
             } else if (MODE == 0) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) if (c + j < C) t[i][j] = bf16_bits_to_f32(((const uint16_t*)row)[c + j]);
+                for (int j = 0; j < 3; ++j) if (c + j < C) t[i][j] = bf16_bits_to_f32(((const uint16_t*)row)[c + j]);
             }
         }
     }
@@ -60,9 +63,10 @@ template <int MODE, bool PAST>
 __device__ __forceinline__ void rn_store_bf16(char* row, int lane, int i, int C, u32x2_t r) {
     const int c = (lane + 64 * i) * 4;
     if (MODE == 2 || (MODE == 1 && c < C)) fw_store<PAST>(row + lane * 8 + i * 512, r);
+    else if (MODE == 0 && c + 4 <= C) *(u32x2_odd_t*)(row + lane * 8 + i * 512) = r;
     else if (MODE == 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) if (c + j < C) ((uint16_t*)row)[c + j] = (uint16_t)(r[j >> 1] >> (16 * (j & 1)));
+        for (int j = 0; j < 3; ++j) if (c + j < C) ((uint16_t*)row)[c + j] = (uint16_t)(r[j >> 1] >> (16 * (j & 1)));
     }
 }
 
@@ -145,9 +149,10 @@ __device__ __forceinline__ void rn_update(const RnArgs& p, const RnParams<VPL, M
         for (int i = 0; i < G; ++i) {
             const int c = (lane + 64 * (i0 + i)) * 4;
             if (MODE == 2 || (MODE == 1 && c < C)) fw_store<PAST>(xo + lane * 16 + (i0 + i) * 1024, v[i]);
+            else if (MODE == 0 && c + 4 <= C) *(f32x4_odd_t*)(xo + lane * 16 + (i0 + i) * 1024) = v[i];
             else if (MODE == 0) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) if (c + j < C) ((float*)xo)[c + j] = v[i][j];
+                for (int j = 0; j < 3; ++j) if (c + j < C) ((float*)xo)[c + j] = v[i][j];
             }
         }
     } else {
