@@ -314,7 +314,15 @@ __global__ __launch_bounds__(POST ? 256 : 512, POST ? 1 : 2) void residual_norm_
         const float* src = rn_ptr(p, k);
         if (!src) continue;
         src += k >= RN_G1 ? (int64_t)g * p.C : 0;
-        for (int i = threadIdx.x; i < VPL * 64; i += T) rn_smem[slot * VPL * 64 + i] = i * 4 < p.C ? *(const f32x4_t*)(src + i * 4) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int i = threadIdx.x; i < VPL * 64; i += T) {
+            f32x4_t t = {0.f, 0.f, 0.f, 0.f};
+            if (MODE > 0 ? i * 4 < p.C : i * 4 + 4 <= p.C) t = MODE > 0 ? *(const f32x4_t*)(src + i * 4) : (f32x4_t)*(const f32x4_odd_t*)(src + i * 4);
+            else if (MODE == 0) {
+#pragma unroll
+                for (int j = 0; j < 3; ++j) if (i * 4 + j < p.C) t[j] = src[i * 4 + j];
+            }
+            rn_smem[slot * VPL * 64 + i] = t;
+        }
         ++slot;
     }
     __syncthreads();
@@ -331,7 +339,8 @@ template <int VPL, int MODE, bool POST>
 int rn_launch(const RnArgs& p, hipStream_t st) {
     // staged from 4096 rows on (a chip full of work-groups walks at least two rows a wave there; below, filling LDS costs more than it
     // saves), if the vectors leave room for it.  Rows past 5120 columns do not fit a wave's registers next to the addressing.
-    if constexpr (MODE > 0 && VPL <= 20) {
+    // Unaligned rows: from 2049 columns on (20001 x 5117: 406 us, 333 staged; 9000 x 1283: 45, 50 staged).
+    if constexpr (VPL <= 20 && (MODE > 0 || VPL == 20)) {
         int vecs = 0;
         for (const float* v : {p.bias, p.post_w, p.w, p.b, p.g1, p.g0, p.scale, p.shift}) vecs += v != nullptr;
         const int lds = vecs * VPL * 64 * 16;

@@ -257,3 +257,16 @@ def test_streams_larger_than_the_caches(ops, xdt, post):
         assert torch.equal(q.q[a:a + 5000], ops.quantize_mxfp4_rows(want).q)
     src = x.clone()
     assert torch.equal(ops.residual_norm(x, y, post=post, **v), h) and torch.equal(x, xo) and not torch.equal(x, src)
+
+
+@pytest.mark.parametrize("out", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("rows,C,groups", [(4103, 2087, 1), (4104, 5119, 3), (4100, 1282, 2), (300, 4097, 1)])
+def test_rows_of_odd_length(ops, rows, C, groups, out):
+    """Rows and vectors that start at any element, with 1, 2 or 3 values behind the last four, from 2049 columns on with staged vectors; in
+    slices of wider rows, what lies beside them stays."""
+    wide, ywide = rnd(rows, C + 6, seed=1, scale=2.0), rnd(rows, C + 7, seed=2, dtype=torch.bfloat16)
+    before = wide.clone()
+    check(ops, wide[:, 3:C + 3], ywide[:, 5:C + 5], out=out, **vectors(C, groups))
+    assert torch.equal(wide[:, :3], before[:, :3]) and torch.equal(wide[:, C + 3:], before[:, C + 3:])
+    xb = before[:, :C].bfloat16()
+    check(ops, xb, ywide[:, :C], out=out, post="layer", norm="rms", **vectors(C, groups, post="layer"))
