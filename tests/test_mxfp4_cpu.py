@@ -52,15 +52,15 @@ def test_product_refusals(lib, p):
 
 
 def test_whole_linear_refusals(lib, p):
-    base = dict(x=p(), ldx=64, W=p(), ldw=128, sw=p(), C=p(), ldc=64, odt=1, cs=None, M=20, N=64, K=64, bias=None, act=0, g1=None, g0=None, res=None, ldr=0, rdt=0, ws=p(), n=1 << 20, st=None)
+    base = dict(x=p(), ldx=64, W=p(), ldw=128, sw=p(), C=p(), ldc=64, odt=1, cs=None, M=40, N=64, K=64, bias=None, act=0, g1=None, g0=None, res=None, ldr=0, rdt=0, ws=p(), n=1 << 20, st=None)
     f = lambda **k: lib.fw_linear_mxfp4(*[k.get(n, v) for n, v in base.items()])
     assert lib.fw_linear_mxfp4_workspace_bytes(20, 64) == 20 * 128 + 256 and lib.fw_linear_mxfp4_workspace_bytes(33, 257) == 33 * 256 + 2 * 512
     assert lib.fw_linear_mxfp4_workspace_bytes(0, 64) == 0 and lib.fw_linear_mxfp4_workspace_bytes(4, 0) == 0
     assert lib.fw_linear_mxfp4_workspace_bytes(1 << 20, 13824) == (1 << 20) * 54 * 128 + (1 << 15) * 54 * 256
-    for bad in (dict(x=None), dict(ldx=63), dict(x=p(1)), dict(ws=None, n=0), dict(n=20 * 128 + 255), dict(ws=p(8)),
-                dict(M=4, K=63, ws=None, n=0), dict(M=4, ldx=65, ws=None, n=0), dict(M=4, x=p(2), ws=None, n=0)):
+    for bad in (dict(x=None), dict(ldx=63), dict(x=p(1)), dict(ws=None, n=0), dict(n=40 * 128 + 511), dict(ws=p(8)),
+                dict(M=20, K=63, ws=None, n=0), dict(M=4, K=63, ws=None, n=0), dict(M=4, ldx=65, ws=None, n=0), dict(M=4, x=p(2), ws=None, n=0)):
         refused(lib, f(**bad), "fw_linear_mxfp4")
-    for m in (4, 20):                       # one launch or two: the product's own refusals come first
+    for m in (4, 20, 40):                    # one launch or two: the product's own refusals come first
         for bad in (dict(W=None), dict(ldw=112), dict(C=None), dict(act=9), dict(odt=0), dict(ldc=63), dict(odt=3), dict(rdt=1), dict(g1=p(2)), dict(K=0), dict(sw=p(1))):
             refused(lib, f(M=m, **bad), "fw_gemm_mxfp4" if "K" not in bad or m == 4 else "")
     assert f(M=0) == 0 and f(N=0) == 0
