@@ -648,7 +648,7 @@ int mx_launch_ring(MxArgs& p, int n_cover, hipStream_t st) {
 //     64 x 128     300   2500            24.0                 82.2                 116.6                 1873
 //     64 x 256     560   5000            28.6                 75.5                 119.6                 1830
 //     128 x 256    950   7500            22.3                103.5                  95.2                 1453
-//     256 x 256   1550  11000            31.5                102.7                  82.0                 1270
+//     256 x 256   1550  11000            31.5                102.7                  82.0                 1190
 // All of them add the same instructions in the same order per output element: a row's bits do not depend on the choice.
 int mx_tile_choice(int M, int n_cover, int slabs) {
     static const int shape[4][4] = {{64, 128, 300, 2500}, {64, 256, 560, 5000}, {128, 256, 950, 7500}, {256, 256, 1550, 11000}};
