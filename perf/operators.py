@@ -9,7 +9,7 @@
 `own` False: plain torch, in 32 bits.  `own` True: the calls of fantasy_world_amd.hip_ops.HipOps.
 
 MXFP4 as used here: the scale byte of a block is the exponent of its largest magnitude minus 2, one more where that magnitude has a
-mantissa of 1.75 or above (it would round past 6, the largest e2m1 value), within 0 (2^-127) and 252 (2^125); values round to the nearest, ties to
+mantissa of 1.75 or above (it would round past 6, the largest e2m1 value), and never below 0 (2^-127); values round to the nearest, ties to
 the even code.  Rows are packed two values a byte, the first in the low half, and padded with zeros to a multiple of 256 values; scale bytes
 lie as [rows / 32][K / 256][32][8]: the 8 scales that a row needs for 256 values next to those of its 31 neighbours.
 """
@@ -148,7 +148,7 @@ def _codes(x):
     rows, K = x.shape
     v = torch.nn.functional.pad(x.float(), (0, -K % 256)).view(rows, -1, 32)
     top = v.abs().amax(2).view(torch.int32)
-    byte = ((top >> 23) - 2 + ((top & 0x7fffff) >= 0x600000)).clamp(0, 252)
+    byte = ((top >> 23) - 2 + ((top & 0x7fffff) >= 0x600000)).clamp(min=0)
     byte = torch.where((top >> 23) == 255, 255, byte)                     # infinities and NaN: the scale is NaN
     a = v.abs().double() * torch.exp2(127.0 - byte.double()).unsqueeze(2)
     code = (a > 0.25).byte() + (a >= 0.75).byte() + (a > 1.25).byte() + (a >= 1.75).byte() + (a > 2.5).byte() + (a >= 3.5).byte() + (a > 5).byte()
@@ -299,7 +299,7 @@ def _round64(x):
     for k in range(0, x.shape[1], 32):
         v = x[:, k:k + 32].double()
         m, e = torch.frexp(v.abs().amax(1, keepdim=True))                # m in [1/2, 1)
-        unit = torch.exp2((e - 3 + (m >= 0.875)).clamp(-127, 125).double())      # exact: pow(2, n) is not, on a GPU
+        unit = torch.ldexp(torch.ones_like(m), (e - 3 + (m >= 0.875)).clamp(min=-127))
         a = v / unit
         step = torch.where(a.abs() < 2, 0.5, torch.where(a.abs() < 4, 1.0, 2.0))
         out[:, k:k + 32] = (torch.round(a / step) * step).clamp(-6, 6) * unit
@@ -313,7 +313,7 @@ def _weights64(w):
     out = torch.empty(N, w["q"].shape[1] * 2, dtype=torch.float64, device=DEV)
     for first, code in ((0, w["q"] % 16), (1, w["q"] // 16)):
         out[:, first::2] = half[(code % 8).long()] * torch.where(code >= 8, -1.0, 1.0).double()
-    return (out * torch.exp2(byte.double() - 127).repeat_interleave(32, 1))[:, :K]
+    return (out * torch.pow(2.0, byte.double() - 127).repeat_interleave(32, 1))[:, :K]
 
 
 def _act64(v, act):
