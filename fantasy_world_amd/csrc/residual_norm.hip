@@ -327,7 +327,7 @@ __global__ __launch_bounds__(POST ? 256 : 512, POST ? 1 : 2) void residual_norm_
     }
     __syncthreads();
     const unsigned last = (unsigned)min((int64_t)p.rows, (int64_t)(g + 1) * p.rows_per_mod);
-    for (unsigned r = (unsigned)(g * p.rows_per_mod + w * (T / 64) + wave); r < last; r += wgs_per_run * (T / 64)) {
+    for (unsigned r = (unsigned)(g * p.rows_per_mod) + w * (T / 64) + wave; r < last; r += wgs_per_run * (T / 64)) {
         // the vectors stay in LDS: as invariants of this loop the compiler keeps them in 320 registers and spills
         int z = 0;
         asm volatile("" : "+s"(z));
@@ -344,11 +344,11 @@ int rn_launch(const RnArgs& p, hipStream_t st) {
         int vecs = 0;
         for (const float* v : {p.bias, p.post_w, p.w, p.b, p.g1, p.g0, p.scale, p.shift}) vecs += v != nullptr;
         const int lds = vecs * VPL * 64 * 16;
-        const int runs = (p.rows + p.rows_per_mod - 1) / p.rows_per_mod;
+        const int runs = (p.rows - 1) / p.rows_per_mod + 1;
         if (vecs && p.rows >= 4096 && runs <= 64 && lds <= 160 * 1024) {
             constexpr int waves = POST ? 4 : 8;
             const int per_cu = POST ? (lds <= 40 * 1024 ? 4 : lds <= 80 * 1024 ? 2 : 1) : (lds <= 80 * 1024 ? 2 : 1);
-            const int wgs_per_run = min(256 * per_cu / runs, (min(p.rows, p.rows_per_mod) + waves - 1) / waves);
+            const int wgs_per_run = min(256 * per_cu / runs, (p.rows_per_mod - 1) / waves + 1);
             const bool past = MODE == 2 && (int64_t)p.rows * p.C * (p.x_dtype == FW_DT_F32 ? 4 : 2) > FW_CACHE_BYTES;
             const auto f = past ? residual_norm_staged_kernel<VPL, MODE, POST, MODE == 2> : residual_norm_staged_kernel<VPL, MODE, POST, false>;
             if (lds > 64 * 1024) {
@@ -359,7 +359,7 @@ int rn_launch(const RnArgs& p, hipStream_t st) {
             return (int)hipGetLastError();
         }
     }
-    hipLaunchKernelGGL((residual_norm_kernel<VPL, MODE, POST>), dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((residual_norm_kernel<VPL, MODE, POST>), dim3((unsigned)((p.rows - 1) / 4 + 1)), dim3(256), 0, st, p);
     return (int)hipGetLastError();
 }
 
@@ -394,7 +394,8 @@ extern "C" int fw_residual_norm(const void* x, int64_t ldx, void* x_out, int64_t
     RnArgs p;
     p.x = x; p.ldx = ldx; p.xo = x_out; p.ldxo = ldxo; p.x_dtype = x_dtype; p.y = y; p.ldy = ldy; p.y_dtype = y_dtype;
     p.bias = bias; p.g1 = g1; p.g0 = g0; p.post = post; p.post_w = post_w; p.norm = norm; p.w = w; p.b = b; p.scale = scale; p.shift = shift;
-    p.eps = eps; p.h = h; p.ldh = ldh; p.hs = h_scale; p.mx = h_dtype == FW_DT_MXFP4; p.slabs = slabs; p.rows = rows; p.C = C; p.rows_per_mod = rows_per_mod;
+    p.eps = eps; p.h = h; p.ldh = ldh; p.hs = h_scale; p.mx = h_dtype == FW_DT_MXFP4; p.slabs = slabs; p.rows = rows; p.C = C;
+    p.rows_per_mod = min(rows_per_mod, rows);            // one vector for all: any value from rows on, the largest int too; sums with it stay in 32 bits
     // 4 values at a time: every row of every operand starts on the access size (16 bytes in fp32, 8 in bf16)
     auto rows_ok = [](const void* q, int64_t ld, int e) { return (((uintptr_t)q) & (4 * e - 1)) == 0 && (ld % 4) == 0; };
     const bool vec = (C % 4) == 0 && (pv & 15) == 0 && rows_ok(x, ldx, xe) && (!y || (rows_ok(y, ldy, ye) && rows_ok(x_out, ldxo, xe))) && (p.mx || rows_ok(h, ldh, 2));
