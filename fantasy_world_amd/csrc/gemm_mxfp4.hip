@@ -52,14 +52,16 @@ __device__ __forceinline__ void mx_tile(const MxArgs& p, int& tm, int& tn) {
 }
 
 // GELU with erf by Abramowitz & Stegun 7.1.26 (|error of erf| <= 1.5e-7), in its complementary form: no cancellation for negative values.
-// erff in its place costs 14 us per 128 x 256 tile.
+// erff in its place costs 14 us per 128 x 256 tile.  Past 8 the value is x itself in fp32 (1 - Phi(8) = 6e-16), infinity included, where the
+// difference below would be inf - inf * 0; at -infinity the formula is -inf * 0, a NaN, here as there.
 __device__ __forceinline__ float mx_gelu_erf(float x) {
     const float z = fabsf(x) * 0.7071067811865476f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
     float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
     q = __builtin_fmaf(q, t, 1.421413741f);
     q = __builtin_fmaf(q, t, -0.284496736f);
     q = __builtin_fmaf(q, t, 0.254829592f);
-    return fmaxf(x, 0.f) - 0.5f * fabsf(x) * (q * t * __expf(-z * z));
+    const float v = fmaxf(x, 0.f) - 0.5f * fabsf(x) * (q * t * __expf(-z * z));
+    return x > 8.f ? x : v;
 }
 template <int ACT>
 __device__ __forceinline__ float mx_act(float v) { return ACT == FW_ACT_GELU_ERF ? mx_gelu_erf(v) : fw_apply_act(v, ACT); }

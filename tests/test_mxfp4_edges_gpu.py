@@ -1,0 +1,39 @@
+"""-m gpu: the MXFP4 linear where its values, tiles, tails and overlaps have an edge, against the definition in 64 bits."""
+import pytest
+import torch
+
+from test_mxfp4_gpu import act64, bytes_of, close, mx64, product64, rnd
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from fantasy_world_amd.hip_ops import HipOps
+    return HipOps("cuda:0")
+
+
+SPECIAL = [float("inf"), float("-inf"), float("nan"), 3e38, -3e38, 9.0, -9.0, 0.0, -0.0]
+
+
+def same_special(got, want):
+    """Infinities and NaN where the definition has them."""
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isinf(got) * torch.sign(got.double()).nan_to_num(), torch.isinf(want) * torch.sign(want).nan_to_num())
+
+
+# one kernel each: up to 16 and 32 rows (bf16 rows), ring tiles, the 256 x 256 tile
+@pytest.mark.parametrize("M,N,K", [(3, 264, 256), (20, 264, 256), (40, 264, 300), (300, 1032, 512), (4352, 4096, 1024)])
+@pytest.mark.parametrize("act", ["gelu_erf", "gelu_tanh", "silu"])
+def test_activations_at_infinity(ops, M, N, K, act):
+    """Infinite, undefined and very large arguments by way of the bias, whose addition they survive unchanged."""
+    x, w, b = rnd(M, K, seed=1), rnd(N, K, seed=2, scale=K ** -0.5), rnd(N, seed=3, dtype=torch.float32)
+    at = torch.arange(len(SPECIAL)) * 29
+    b[at] = torch.tensor(SPECIAL)
+    lin = ops.pack_linear_mxfp4(w, b)
+    got = ops.linear(x.cuda(), lin, act=act, out_f32=True)
+    v = (mx64(x.cuda())[0] @ mx64(w.cuda())[0].t() + b.double().cuda())
+    same_special(got, act64(v, act))
+    assert torch.isinf(got[:, 0]).all() and (got[:, 0] > 0).all() and torch.isnan(got[:, 58]).all()
+    keep = ~torch.isnan(got)
+    assert torch.equal(ops.linear(x.cuda(), lin, act=act)[keep], got.bfloat16()[keep])
