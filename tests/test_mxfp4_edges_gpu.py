@@ -37,3 +37,21 @@ def test_activations_at_infinity(ops, M, N, K, act):
     assert torch.isinf(got[:, 0]).all() and (got[:, 0] > 0).all() and torch.isnan(got[:, 58]).all()
     keep = ~torch.isnan(got)
     assert torch.equal(ops.linear(x.cuda(), lin, act=act)[keep], got.bfloat16()[keep])
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 264, 256), (20, 264, 256), (40, 264, 300), (300, 1032, 512), (4352, 4096, 1024)])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu_erf", "gelu_tanh", "silu"])
+def test_nan_products_stay_nan_through_the_activation(ops, M, N, K, act):
+    """A row of x and a row of w with an infinity in one block: their whole row and column of the product is NaN, and nothing else is."""
+    x, w = rnd(M, K, seed=1), rnd(N, K, seed=2, scale=K ** -0.5)
+    x[M // 2, 40], w[7, 200] = float("inf"), float("nan")
+    lin = ops.pack_linear_mxfp4(w, rnd(N, seed=3, dtype=torch.float32))
+    want = torch.zeros(M, N, dtype=torch.bool, device="cuda")
+    want[M // 2], want[:, 7] = True, True
+    for kw in (dict(out_f32=True), dict()):
+        assert torch.equal(torch.isnan(ops.linear(x.cuda(), lin, act=act, **kw)), want)
+    # MXFP4 output: the blocks that hold a NaN, and they alone
+    back = ops.dequantize_mxfp4_rows(ops.linear(x.cuda(), lin, act=act, out_mxfp4=True))
+    block = want.clone()
+    block[:, :32] = True
+    assert torch.equal(torch.isnan(back), block)
