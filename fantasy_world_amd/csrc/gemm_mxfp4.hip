@@ -39,6 +39,11 @@ __device__ __forceinline__ auto mx_rsrc(const uint8_t* base, long long bytes) {
     return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(unsigned)(bytes > 0xffffffffLL ? 0xffffffffLL : bytes < 0 ? 0 : bytes), 0x00020000);
 }
 
+// the same over `rows` rows of `slabs` slabs, to the last byte of the last one: the stride's tail behind it need not be anybody's memory
+__device__ __forceinline__ auto mx_rows_rsrc(const uint8_t* base, int rows, int64_t ld, int slabs) {
+    return mx_rsrc(base, rows <= 0 ? 0 : (long long)(rows - 1) * ld + slabs * 128);
+}
+
 // tile of this work-group: XCD-contiguous tile ranges (bijective), groups of GROUP row tiles walked column by column inside them
 __device__ __forceinline__ void mx_tile(const MxArgs& p, int& tm, int& tn) {
     const int nwg = p.tiles_m * p.tiles_n;
@@ -246,7 +251,8 @@ __device__ __forceinline__ void mx_finish(const MxArgs& p, char* reg, const Acc&
 // BM x BN tiles, K slabs of 256 values in a ring of ST stages: four waves multiply (wave tile 32 x 64 at 64 x 128, 64 x 64 at 64 x 256, 128 x 64
 // at 128 x 256), four others do nothing but request codes and scale bytes by LDS-DMA, ST - 1 slabs ahead; one barrier a slab.  A slab past
 // the end is requested out of the descriptors' range (zeros into a stage that nobody reads any more), so the loaders' counted wait is the
-// same number in every iteration.
+// same number in every iteration.  The descriptors end with the last byte of their last row: 255 strides below 2^23 and 2^23 bytes make
+// less than 2^31, and the lane offset of a request past the end starts there.
 // Why loaders of their own: a wave that requests its slab is held until the CU's path from L2 (64 bytes a clock) has taken the request, and
 // with one multiplying wave on a SIMD nobody multiplies meanwhile -- 257 x 5120 x 13824 took 39 us with four waves doing both, at two stages
 // as at four, and takes 21.7 with loaders.  What bounds it now is LDS (the waves' fragment reads and the DMA's writes: 574, 840 and 1150
@@ -268,10 +274,9 @@ __global__ __launch_bounds__(512, ST * (BM + BN) * 136 <= 80 * 1024 ? 4 : 2) voi
     int tm, tn;
     mx_tile(p, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
-    // descriptors of this tile's rows alone: below 2^30 bytes, so PAST lies outside of every one
-    constexpr int PAST = 0x7f000000;
-    const auto ars = mx_rsrc(p.A + (int64_t)m0 * p.lda, (long long)min(p.M - m0, BM) * p.lda);
-    const auto wrs = mx_rsrc(p.W + (int64_t)n0 * p.ldw, (long long)min(p.N - n0, BN) * p.ldw);
+    constexpr unsigned PAST = 0x80000000u;
+    const auto ars = mx_rows_rsrc(p.A + (int64_t)m0 * p.lda, min(p.M - m0, BM), p.lda, p.slabs);
+    const auto wrs = mx_rows_rsrc(p.W + (int64_t)n0 * p.ldw, min(p.N - n0, BN), p.ldw, p.slabs);
     const int sstride = __builtin_amdgcn_readfirstlane(p.slabs * 256);
     const auto sars = mx_rsrc(p.sa + (int64_t)(m0 >> 5) * sstride, (long long)min((p.M + 31) / 32 - (m0 >> 5), BM / 32) * sstride);
     const auto swrs = mx_rsrc(p.sw + (int64_t)(n0 >> 5) * sstride, (long long)min((p.N + 31) / 32 - (n0 >> 5), BN / 32) * sstride);
@@ -280,18 +285,18 @@ __global__ __launch_bounds__(512, ST * (BM + BN) * 136 <= 80 * 1024 ? 4 : 2) voi
     const int vw[2] = {pr * (int)p.ldw + ((pc ^ (pr >> 1)) << 4), pr * (int)p.ldw + ((pc ^ ((pr >> 1) | 4)) << 4)};
     const int astep = __builtin_amdgcn_readfirstlane((int)p.lda * 8), wstep = __builtin_amdgcn_readfirstlane((int)p.ldw * 8);
     auto issue = [&](char* st, int kt) __attribute__((always_inline)) {
-        const int k0 = kt < p.slabs ? kt * 128 : PAST, s0 = kt < p.slabs ? kt * 256 : PAST;
-        const int live = kt < p.slabs ? 1 : 0;
+        const int k0 = kt * 128, s0 = kt * 256;
+        const int live = kt < p.slabs ? -1 : 0, past = (int)PAST & ~live;
 #pragma unroll
-        for (int j = 0; j < APC; ++j) FWX_BLDS16(ars, va[j & 1], k0 + live * (wave * APC + j) * astep, st + (wave * APC + j) * 1024);
+        for (int j = 0; j < APC; ++j) FWX_BLDS16(ars, va[j & 1] | past, (k0 + (wave * APC + j) * astep) & live, st + (wave * APC + j) * 1024);
 #pragma unroll
-        for (int j = 0; j < WPC; ++j) FWX_BLDS16(wrs, vw[j & 1], k0 + live * (wave * WPC + j) * wstep, st + BM * 128 + (wave * WPC + j) * 1024);
+        for (int j = 0; j < WPC; ++j) FWX_BLDS16(wrs, vw[j & 1] | past, (k0 + (wave * WPC + j) * wstep) & live, st + BM * 128 + (wave * WPC + j) * 1024);
 #pragma unroll
         for (int j = 0; j < SPC; ++j) {
             const int g = min(wave + 4 * j, RB - 1);
             char* d = st + (BM + BN) * 128 + g * 256;
-            if (g < BM / 32) __builtin_amdgcn_raw_ptr_buffer_load_lds(sars, FW_LDS_PTR(d), 4, lane * 4, s0 + live * g * sstride, 0, 0);
-            else __builtin_amdgcn_raw_ptr_buffer_load_lds(swrs, FW_LDS_PTR(d), 4, lane * 4, s0 + live * (g - BM / 32) * sstride, 0, 0);
+            if (g < BM / 32) __builtin_amdgcn_raw_ptr_buffer_load_lds(sars, FW_LDS_PTR(d), 4, lane * 4 | past, (s0 + g * sstride) & live, 0, 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(swrs, FW_LDS_PTR(d), 4, lane * 4 | past, (s0 + (g - BM / 32) * sstride) & live, 0, 0);
         }
     };
     const int swz = (fi >> 1) & 7;
@@ -366,8 +371,8 @@ __global__ __launch_bounds__(512, 2) void gemm_mxfp4_256_kernel(MxArgs p) {
     int tm, tn;
     mx_tile(p, tm, tn);
     const int m0 = tm * LM, n0 = tn * LN;
-    const auto ars = mx_rsrc(p.A + (int64_t)m0 * p.lda, (long long)(p.M - m0) * p.lda);
-    const auto wrs = mx_rsrc(p.W + (int64_t)n0 * p.ldw, (long long)(p.N - n0) * p.ldw);
+    const auto ars = mx_rows_rsrc(p.A + (int64_t)m0 * p.lda, min(p.M - m0, LM), p.lda, p.slabs);
+    const auto wrs = mx_rows_rsrc(p.W + (int64_t)n0 * p.ldw, min(p.N - n0, LN), p.ldw, p.slabs);
     // scale tiles of this wave's 4 + 2 groups of 32 rows; groups past the end read zeros
     const int sstride = __builtin_amdgcn_readfirstlane(p.slabs * 256);
     const int ab = (m0 >> 5) + grp * 4, wb = (n0 >> 5) + wn * 2;

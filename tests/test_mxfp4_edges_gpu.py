@@ -55,3 +55,22 @@ def test_nan_products_stay_nan_through_the_activation(ops, M, N, K, act):
     block = want.clone()
     block[:, :32] = True
     assert torch.equal(torch.isnan(back), block)
+
+
+@pytest.mark.parametrize("M", [3, 40, 1000])
+def test_strides_up_to_the_limit(ops, M):
+    """Weight rows almost 2^23 bytes apart, the last row ending with its buffer; activation rows the same way.  The result is that of
+    close rows."""
+    N, K, ld = 256, 300, (1 << 23) - 16
+    x, wm = rnd(M, K, seed=1).cuda(), ops.quantize_mxfp4_rows(rnd(N, K, seed=2, scale=K ** -0.5).cuda())
+    mx = ops.quantize_mxfp4_rows(x)
+    want = ops.linear(mx, ops.linear_from_mxfp4(wm.q, wm.s, None, K))
+    from fantasy_world_amd.hip_ops import MXFP4Rows
+
+    def spread(rows):
+        n, width = rows.shape
+        far = torch.empty((n - 1) * ld + width, dtype=torch.uint8, device="cuda").as_strided((n, width), (ld, 1))
+        far.copy_(rows)
+        return far
+    assert torch.equal(want, ops.linear(mx, ops.linear_from_mxfp4(spread(wm.q), wm.s, None, K)))
+    assert torch.equal(want, ops.linear(MXFP4Rows(spread(mx.q), mx.s, K), ops.linear_from_mxfp4(wm.q, wm.s, None, K)))
