@@ -702,6 +702,7 @@ bool mx_rows_fused(const void* x, int64_t ldx, int M, int K) {
 // Everything but A: the checks that fw_gemm_mxfp4 and fw_linear_mxfp4 share, and the arguments.  0, or the error code with its message set.
 static int mx_args(MxArgs& p, const uint8_t* W, int64_t ldw, const uint8_t* sw, void* C, int64_t ldc, int out_dtype, uint8_t* cs, int M, int N, int K,
                    const float* bias, int act, const float* g1, const float* g0, const void* res, int64_t ldr, int res_dtype) {
+    if (M > MX_MAX || N > MX_MAX || K > MX_MAX) { fw_set_error("fw_gemm_mxfp4: M, N and K below 2^31 - 256 required"); return FW_E_BADARG; }
     const int slabs = mx_slabs(K), cslabs = mx_slabs(N);
     if (!W || !sw || !C || K <= 0 || ldw < (int64_t)slabs * 128 || (ldw % 16) || ldw >= (1 << 23) || (((uintptr_t)W) & 15) || (((uintptr_t)sw) & 3)) {
         fw_set_error("fw_gemm_mxfp4: K > 0; W 16-byte aligned with roundup(K, 256) / 2 <= ldw < 2^23, ldw % 16 == 0; scales 4-byte aligned"); return FW_E_BADARG; }
@@ -769,7 +770,7 @@ extern "C" int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, c
 extern "C" int64_t fw_linear_mxfp4_workspace_bytes(int M, int K) {
     if (M <= 0 || K <= 0) return 0;
     const int64_t slabs = mx_slabs(K);
-    return (int64_t)M * slabs * 128 + (int64_t)((M + 31) / 32) * slabs * 256;
+    return (int64_t)M * slabs * 128 + ((int64_t)M + 31) / 32 * slabs * 256;
 }
 
 extern "C" int fw_linear_mxfp4(const uint16_t* x, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* sw,

@@ -19,7 +19,10 @@
 
 constexpr int MX_SLAB = 256;                 // values of one padded K slab = 128 bytes of codes + 8 scale bytes a row
 
-static inline int mx_slabs(int K) { return (K + MX_SLAB - 1) / MX_SLAB; }
+// largest number of values of a row (and of rows of a product): whole slabs and tiles of it are still counted in 32 bits
+constexpr int MX_MAX = 0x7fffffff - MX_SLAB;
+
+static inline int mx_slabs(int K) { return (int)(((int64_t)K + MX_SLAB - 1) / MX_SLAB); }
 
 // scale byte from the fp32 bits of the largest magnitude (taken by integer compare: NaN sorts above infinity)
 __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {

@@ -124,11 +124,11 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_rows_kernel(const uint8_t* 
 extern "C" int fw_mxfp4_quant_rows(const void* x, int64_t ldx, int x_dtype, uint8_t* q, int64_t ldq, uint8_t* s, int M, int K, void* stream) {
     if (M <= 0) return 0;
     const int slabs = mx_slabs(K);
-    if (!x || !q || !s || K <= 0 || ldx < K || ldq < (int64_t)slabs * 128 || (ldq % 16) || (((uintptr_t)q) & 15) || (((uintptr_t)s) & 3) ||
+    if (!x || !q || !s || K <= 0 || K > MX_MAX || ldx < K || ldq < (int64_t)slabs * 128 || (ldq % 16) || (((uintptr_t)q) & 15) || (((uintptr_t)s) & 3) ||
         (x_dtype != FW_DT_BF16 && x_dtype != FW_DT_F32) || (((uintptr_t)x) & (x_dtype == FW_DT_F32 ? 3 : 1))) {
-        fw_set_error("fw_mxfp4_quant_rows: bf16 / f32 x with ldx >= K > 0, q 16-byte aligned with ldq % 16 == 0 and ldq >= roundup(K, 256) / 2, s 4-byte aligned required");
+        fw_set_error("fw_mxfp4_quant_rows: bf16 / f32 x with ldx >= K, 0 < K < 2^31 - 256, q 16-byte aligned with ldq % 16 == 0 and ldq >= roundup(K, 256) / 2, s 4-byte aligned required");
         return FW_E_BADARG; }
-    const int64_t nwg = (int64_t)((M + 31) / 32) * slabs;
+    const int64_t nwg = ((int64_t)M + 31) / 32 * slabs;
     if (nwg > 0x7fffffff) { fw_set_error("fw_mxfp4_quant_rows: grid too large"); return FW_E_BADARG; }
     const bool vec = (K % 8) == 0 && ((((uintptr_t)x) & 15) == 0) && (ldx % (x_dtype == FW_DT_F32 ? 4 : 8)) == 0;
     const bool past = (int64_t)M * K * (x_dtype == FW_DT_F32 ? 4 : 2) > FW_CACHE_BYTES;
@@ -149,11 +149,11 @@ extern "C" int fw_mxfp4_quant_rows(const void* x, int64_t ldx, int x_dtype, uint
 extern "C" int fw_mxfp4_dequant_rows(const uint8_t* q, int64_t ldq, const uint8_t* s, void* y, int64_t ldy, int y_dtype, int M, int K, void* stream) {
     if (M <= 0) return 0;
     const int slabs = mx_slabs(K);
-    if (!q || !s || !y || K <= 0 || ldy < K || ldq < (int64_t)slabs * 128 || (ldq % 16) || (((uintptr_t)q) & 15) ||
+    if (!q || !s || !y || K <= 0 || K > MX_MAX || ldy < K || ldq < (int64_t)slabs * 128 || (ldq % 16) || (((uintptr_t)q) & 15) ||
         (y_dtype != FW_DT_BF16 && y_dtype != FW_DT_F32) || (((uintptr_t)y) & (y_dtype == FW_DT_F32 ? 3 : 1))) {
-        fw_set_error("fw_mxfp4_dequant_rows: bf16 / f32 y with ldy >= K > 0, q 16-byte aligned with ldq % 16 == 0 and ldq >= roundup(K, 256) / 2 required");
+        fw_set_error("fw_mxfp4_dequant_rows: bf16 / f32 y with ldy >= K, 0 < K < 2^31 - 256, q 16-byte aligned with ldq % 16 == 0 and ldq >= roundup(K, 256) / 2 required");
         return FW_E_BADARG; }
-    const int64_t nwg = (int64_t)((M + 31) / 32) * slabs;
+    const int64_t nwg = ((int64_t)M + 31) / 32 * slabs;
     if (nwg > 0x7fffffff) { fw_set_error("fw_mxfp4_dequant_rows: grid too large"); return FW_E_BADARG; }
     const bool vec = (K % 8) == 0 && ((((uintptr_t)y) & 15) == 0) && (ldy % (y_dtype == FW_DT_F32 ? 4 : 8)) == 0;
     const bool past = (int64_t)M * K * (y_dtype == FW_DT_F32 ? 4 : 2) > FW_CACHE_BYTES;

@@ -461,7 +461,7 @@ int fw_gemm_fp8(const uint8_t* A, int64_t lda, const uint8_t* W, int64_t ldw, co
  *     it decodes to NaN and every product with it is NaN.
  *   value: e2m1(v / scale), to nearest, ties to the even code; values above 6 scales saturate.
  * Storage ("MXFP4 rows", M x K): codes q [M][ldq] bytes, two values a byte with the first in the low half, K padded with zeros to
- *   Kp = roundup(K, 256): ldq >= Kp / 2, ldq % 16 == 0, q 16-byte aligned; scales s [ceil(M / 32)][Kp / 256][32][8] bytes, contiguous, 4-byte
+ *   Kp = roundup(K, 256), K < 2^31 - 256: ldq >= Kp / 2, ldq % 16 == 0, q 16-byte aligned; scales s [ceil(M / 32)][Kp / 256][32][8] bytes, contiguous, 4-byte
  *   aligned: s[r / 32][k / 256][r % 32][k / 32 % 8].  Scale bytes of the padding past K are not 0xff; those of rows past M are not read as values.
  * ------------------------------------------------------------------------------------------------------------- */
 
@@ -476,7 +476,7 @@ int fw_mxfp4_dequant_rows(const uint8_t* q, int64_t ldq, const uint8_t* s, void*
  * fw_gemm_bf16's epilogue (bias -> act -> per-column affine g1 / g0 -> + residual -> out_dtype).  C may alias res.
  * out_dtype FW_DT_MXFP4: the result is rounded to bf16 and quantised along N by the rule above -- the bytes of fw_mxfp4_quant_rows on the
  * bf16 output -- C = codes [M][ldc] (bytes), cs = scales; the input of the next MXFP4 linear without a pass of its own (cs is not used
- * for the other types).  lda, ldw (bytes) < 2^23.  A row's bits depend on nothing but the row -- except that products of up to 32 rows add
+ * for the other types).  lda, ldw (bytes) < 2^23; M, N < 2^31 - 256.  A row's bits depend on nothing but the row -- except that products of up to 32 rows add
  * their terms in another order than those of more. */
 int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, const uint8_t* W, int64_t ldw, const uint8_t* sw,
                   void* C, int64_t ldc, int out_dtype, uint8_t* cs, int M, int N, int K,
