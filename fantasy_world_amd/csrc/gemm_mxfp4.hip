@@ -699,6 +699,23 @@ bool mx_rows_fused(const void* x, int64_t ldx, int M, int K) {
 
 }  // namespace
 
+// Work-groups read all of the operands while others store: an output shares no byte with any of them.  The residual is read by the lane
+// that stores in its place, so C may be the residual -- the same rows in the same type.
+static bool mx_overlap(const MxArgs& p, const FwSpan& a, const FwSpan& a_scale) {
+    const int ce = p.out_dtype == FW_DT_F32 ? 4 : 2, re = p.res_dtype == FW_DT_F32 ? 4 : 2;
+    const bool mx = p.out_dtype == FW_DT_MXFP4;
+    const FwSpan c = mx ? FwSpan(p.C, p.ldc, (int64_t)p.cslabs * 128, p.M) : FwSpan(p.C, p.ldc * ce, (int64_t)p.N * ce, p.M);
+    const FwSpan cs(mx ? p.cs : nullptr, ((int64_t)p.M + 31) / 32 * p.cslabs * 256), res(p.res_dtype == FW_DT_NONE ? nullptr : p.res, p.ldr * re, (int64_t)p.N * re, p.M);
+    const FwSpan in[] = {a, a_scale, FwSpan(p.W, p.ldw, (int64_t)p.slabs * 128, p.N), FwSpan(p.sw, ((int64_t)p.N + 31) / 32 * p.slabs * 256),
+                         FwSpan(p.bias, (int64_t)p.N * 4), FwSpan(p.g1, (int64_t)p.N * 4), FwSpan(p.g0, (int64_t)p.N * 4)};
+    for (const FwSpan& i : in) if (fw_overlap(i, c) || fw_overlap(i, cs)) return true;
+    return fw_overlap(c, cs) || fw_overlap(res, cs) || (fw_overlap(res, c) && !(res.same(c) && p.res_dtype == p.out_dtype));
+}
+static int mx_refuse_overlap() {
+    fw_set_error("fw_gemm_mxfp4: the output overlaps an operand (it may be the residual: the same rows in the same type)");
+    return FW_E_BADARG;
+}
+
 // Everything but A: the checks that fw_gemm_mxfp4 and fw_linear_mxfp4 share, and the arguments.  0, or the error code with its message set.
 static int mx_args(MxArgs& p, const uint8_t* W, int64_t ldw, const uint8_t* sw, void* C, int64_t ldc, int out_dtype, uint8_t* cs, int M, int N, int K,
                    const float* bias, int act, const float* g1, const float* g0, const void* res, int64_t ldr, int res_dtype) {
@@ -737,6 +754,7 @@ extern "C" int fw_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint8_t* sa, c
     if (!A || !sa || lda < (int64_t)slabs * 128 || (lda % 16) || lda >= (1 << 23) || (((uintptr_t)A) & 15) || (((uintptr_t)sa) & 3)) {
         fw_set_error("fw_gemm_mxfp4: A 16-byte aligned with roundup(K, 256) / 2 <= lda < 2^23, lda % 16 == 0; scales 4-byte aligned"); return FW_E_BADARG; }
     p.A = A; p.lda = lda; p.sa = sa;
+    if (mx_overlap(p, FwSpan(A, lda, (int64_t)slabs * 128, M), FwSpan(sa, ((int64_t)M + 31) / 32 * slabs * 256))) return mx_refuse_overlap();
     const int n_cover = out_dtype == FW_DT_MXFP4 ? cslabs * MX_SLAB : N;       // the padding of a quantised row is written too
     hipStream_t st = (hipStream_t)stream;
     if (M <= 16) return mx_launch_rows<1, false>(p, n_cover, 0, st);
@@ -783,6 +801,7 @@ extern "C" int fw_linear_mxfp4(const uint16_t* x, int64_t ldx, const uint8_t* W,
         MxArgs p;
         if (const int rc = mx_args(p, W, ldw, sw, C, ldc, out_dtype, cs, M, N, K, bias, act, g1, g0, res, ldr, res_dtype)) return rc;
         p.A = (const uint8_t*)x; p.lda = ldx * 2; p.sa = nullptr;
+        if (mx_overlap(p, FwSpan(x, ldx * 2, (int64_t)K * 2, M), FwSpan(nullptr, 0))) return mx_refuse_overlap();
         const int n_cover = out_dtype == FW_DT_MXFP4 ? p.cslabs * MX_SLAB : N;
         return M <= 16 ? mx_launch_rows<1, true>(p, n_cover, K / 32, (hipStream_t)stream) : mx_launch_rows<2, true>(p, n_cover, K / 32, (hipStream_t)stream);
     }
@@ -794,6 +813,7 @@ extern "C" int fw_linear_mxfp4(const uint16_t* x, int64_t ldx, const uint8_t* W,
     // the product's arguments first: nothing is launched for a call that is refused
     MxArgs p;
     if (const int rc = mx_args(p, W, ldw, sw, C, ldc, out_dtype, cs, M, N, K, bias, act, g1, g0, res, ldr, res_dtype)) return rc;
+    if (mx_overlap(p, FwSpan(x, ldx * 2, (int64_t)K * 2, M), FwSpan(workspace, fw_linear_mxfp4_workspace_bytes(M, K)))) return mx_refuse_overlap();
     if (const int rc = fw_mxfp4_quant_rows(x, ldx, FW_DT_BF16, q, lda, s, M, K, stream)) return rc;
     return fw_gemm_mxfp4(q, lda, s, W, ldw, sw, C, ldc, out_dtype, cs, M, N, K, bias, act, g1, g0, res, ldr, res_dtype, stream);
 }

@@ -24,6 +24,35 @@ constexpr int MX_MAX = 0x7fffffff - MX_SLAB;
 
 static inline int mx_slabs(int K) { return (int)(((int64_t)K + MX_SLAB - 1) / MX_SLAB); }
 
+// Operands as the host sees them: `rows` rows of `width` bytes, `pitch` bytes apart (pitch >= width).  Absent ones have no rows.
+struct FwSpan {
+    uintptr_t at; int64_t pitch, width, rows;
+    FwSpan(const void* p, int64_t pitch_, int64_t width_, int64_t rows_) : at((uintptr_t)p), pitch(pitch_), width(width_), rows(p && width_ > 0 ? rows_ : 0) {}
+    FwSpan(const void* p, int64_t bytes) : FwSpan(p, bytes, bytes, 1) {}
+    bool same(const FwSpan& o) const { return at == o.at && width == o.width && rows == o.rows && (pitch == o.pitch || rows == 1); }
+    int64_t end() const { return (int64_t)at + (rows - 1) * pitch + width; }
+};
+
+// Do two operands share a byte?  Column slices of one buffer interleave without sharing any: equal pitches are decided by the distance
+// modulo the pitch, others row by row.
+static inline bool fw_overlap(const FwSpan& a, const FwSpan& b) {
+    if (a.rows <= 0 || b.rows <= 0 || a.end() <= (int64_t)b.at || b.end() <= (int64_t)a.at) return false;
+    if (a.rows > b.rows) return fw_overlap(b, a);
+    const int64_t d = (int64_t)a.at - (int64_t)b.at, P = b.pitch;
+    auto floor_div = [](int64_t n, int64_t m) { return n / m - (n % m < 0 ? 1 : 0); };
+    if (a.pitch == P) {
+        // row i of a starts r bytes into pitch i + k of b
+        const int64_t k = floor_div(d, P), r = d - k * P;
+        auto meet = [&](int64_t s) { return (s > 0 ? s : 0) < (b.rows < a.rows + s ? b.rows : a.rows + s); };      // some i with 0 <= i + s < b.rows
+        return (r < b.width && meet(k)) || (r + a.width > P && meet(k + 1));
+    }
+    for (int64_t i = 0; i < a.rows; ++i) {
+        const int64_t s = d + i * a.pitch, j = floor_div(s - b.width, P) + 1;                     // the first row of b that ends behind s
+        if ((j > 0 ? j : 0) < b.rows && (j > 0 ? j : 0) * P < s + a.width) return true;
+    }
+    return false;
+}
+
 // scale byte from the fp32 bits of the largest magnitude (taken by integer compare: NaN sorts above infinity)
 __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
     const uint32_t e = top >> 23;

@@ -130,6 +130,9 @@ extern "C" int fw_mxfp4_quant_rows(const void* x, int64_t ldx, int x_dtype, uint
         return FW_E_BADARG; }
     const int64_t nwg = ((int64_t)M + 31) / 32 * slabs;
     if (nwg > 0x7fffffff) { fw_set_error("fw_mxfp4_quant_rows: grid too large"); return FW_E_BADARG; }
+    const FwSpan xs(x, ldx * (x_dtype == FW_DT_F32 ? 4 : 2), (int64_t)K * (x_dtype == FW_DT_F32 ? 4 : 2), M), qs(q, ldq, (int64_t)slabs * 128, M);
+    const FwSpan ss(s, ((int64_t)M + 31) / 32 * slabs * 256);
+    if (fw_overlap(xs, qs) || fw_overlap(xs, ss) || fw_overlap(qs, ss)) { fw_set_error("fw_mxfp4_quant_rows: x, q and s must not overlap"); return FW_E_BADARG; }
     const bool vec = (K % 8) == 0 && ((((uintptr_t)x) & 15) == 0) && (ldx % (x_dtype == FW_DT_F32 ? 4 : 8)) == 0;
     const bool past = (int64_t)M * K * (x_dtype == FW_DT_F32 ? 4 : 2) > FW_CACHE_BYTES;
     const dim3 g((unsigned)nwg), b(256);
@@ -155,6 +158,9 @@ extern "C" int fw_mxfp4_dequant_rows(const uint8_t* q, int64_t ldq, const uint8_
         return FW_E_BADARG; }
     const int64_t nwg = ((int64_t)M + 31) / 32 * slabs;
     if (nwg > 0x7fffffff) { fw_set_error("fw_mxfp4_dequant_rows: grid too large"); return FW_E_BADARG; }
+    const FwSpan ys(y, ldy * (y_dtype == FW_DT_F32 ? 4 : 2), (int64_t)K * (y_dtype == FW_DT_F32 ? 4 : 2), M);
+    if (fw_overlap(ys, FwSpan(q, ldq, (int64_t)slabs * 128, M)) || fw_overlap(ys, FwSpan(s, ((int64_t)M + 31) / 32 * slabs * 256))) {
+        fw_set_error("fw_mxfp4_dequant_rows: y must not overlap q or s"); return FW_E_BADARG; }
     const bool vec = (K % 8) == 0 && ((((uintptr_t)y) & 15) == 0) && (ldy % (y_dtype == FW_DT_F32 ? 4 : 8)) == 0;
     const bool past = (int64_t)M * K * (y_dtype == FW_DT_F32 ? 4 : 2) > FW_CACHE_BYTES;
     const dim3 g((unsigned)nwg), b(256);

@@ -391,6 +391,23 @@ extern "C" int fw_residual_norm(const void* x, int64_t ldx, void* x_out, int64_t
         fw_set_error("fw_residual_norm: bf16 h with ldh >= C, or MXFP4 h with h_scale, 16-byte aligned rows and ldh >= roundup(C, 256) / 2"); return FW_E_BADARG; }
     const uintptr_t pv = ((uintptr_t)bias) | ((uintptr_t)g1) | ((uintptr_t)g0) | ((uintptr_t)post_w) | ((uintptr_t)w) | ((uintptr_t)b) | ((uintptr_t)scale) | ((uintptr_t)shift);
     if (pv & 3) { fw_set_error("fw_residual_norm: misaligned parameter vector"); return FW_E_BADARG; }
+    // A row is whole in its wave's registers before its outputs are stored, so an output may be an input -- the same rows in the same type --
+    // but shares no byte with any other operand, which other waves still read.
+    {
+        const int64_t runs = (rows - 1) / rows_per_mod + 1;
+        const bool mx = h_dtype == FW_DT_MXFP4;
+        const FwSpan xs(x, ldx * xe, (int64_t)C * xe, rows), ys(y, ldy * ye, (int64_t)C * ye, rows), xos(y ? x_out : nullptr, ldxo * xe, (int64_t)C * xe, rows);
+        const FwSpan hs(h, mx ? ldh : ldh * 2, mx ? (int64_t)slabs * 128 : (int64_t)C * 2, rows), ss(mx ? h_scale : nullptr, ((int64_t)rows + 31) / 32 * slabs * 256);
+        auto clash = [](const FwSpan& in, bool same_type, const FwSpan& out) { return fw_overlap(in, out) && !(same_type && in.same(out)); };
+        bool bad = clash(xs, true, xos) || clash(ys, x_dtype == y_dtype, xos) || clash(xs, x_dtype == h_dtype, hs) || clash(ys, y_dtype == h_dtype, hs) ||
+                   fw_overlap(xos, hs) || fw_overlap(xs, ss) || fw_overlap(ys, ss) || fw_overlap(xos, ss) || fw_overlap(hs, ss);
+        const float* vec[] = {bias, post_w, w, b, g1, g0, scale, shift};
+        for (int i = 0; i < 8; ++i) {
+            const FwSpan v(vec[i], (i < 4 ? 1 : runs) * C * 4);
+            bad = bad || fw_overlap(v, xos) || fw_overlap(v, hs) || fw_overlap(v, ss);
+        }
+        if (bad) { fw_set_error("fw_residual_norm: an output overlaps another operand (it may be x or y: the same rows in the same type)"); return FW_E_BADARG; }
+    }
     RnArgs p;
     p.x = x; p.ldx = ldx; p.xo = x_out; p.ldxo = ldxo; p.x_dtype = x_dtype; p.y = y; p.ldy = ldy; p.y_dtype = y_dtype;
     p.bias = bias; p.g1 = g1; p.g0 = g0; p.post = post; p.post_w = post_w; p.norm = norm; p.w = w; p.b = b; p.scale = scale; p.shift = shift;

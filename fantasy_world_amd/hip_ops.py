@@ -797,8 +797,8 @@ class HipOps:
         return lin
 
     def _linear_mxfp4(self, x, lin, act=None, g1=None, g0=None, res=None, out_f32=False, out=None, out_mxfp4=False):
-        """bf16 rows (quantised here) or MXFP4Rows x -> epilogue(x W^T): bf16, fp32 or MXFP4Rows.  out may be res, but not x: work-groups read
-        all of x while others store."""
+        """bf16 rows (quantised here) or MXFP4Rows x -> epilogue(x W^T): bf16, fp32 or MXFP4Rows.  out may be res (the same rows in the same
+        type); otherwise it shares no memory with x, res or the linear: work-groups read all of them while others store."""
         N = lin.N
         ready = isinstance(x, MXFP4Rows)
         if ready:
@@ -870,7 +870,8 @@ class HipOps:
         bf16 rows (h_out: written there, rows may be strided) or (out="mxfp4") MXFP4Rows.  y None: h alone, and the update's arguments are not
         looked at.  x, x_out [rows, C] fp32 or bf16, y fp32 or bf16, C <= 8192; bias / post_w / w / b [C]; g1 / g0 / scale / shift [C], or all
         of them [groups, C] with rows % groups == 0: equal runs of rows share a vector.  post: None, "layer" or "rms" (post_w only with it);
-        norm: "layer" or "rms" (b only with w)."""
+        norm: "layer" or "rms" (b only with w).  x_out and h_out each may be x or y (the same rows in the same type) and otherwise share no
+        memory with the operands or with each other."""
         ldx = self._rows("x", x, torch.float32, torch.bfloat16)
         if out not in ("bf16", "mxfp4") or norm not in ("layer", "rms") or post not in RNORM:
             raise ValueError(f"out: 'bf16' | 'mxfp4', norm: 'layer' | 'rms', post: None | 'layer' | 'rms'; got {out!r}, {norm!r}, {post!r}")

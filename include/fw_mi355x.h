@@ -473,7 +473,8 @@ int fw_mxfp4_quant_rows(const void* x, int64_t ldx, int x_dtype, uint8_t* q, int
 int fw_mxfp4_dequant_rows(const uint8_t* q, int64_t ldq, const uint8_t* s, void* y, int64_t ldy, int y_dtype, int M, int K, void* stream);
 
 /* C[M][N] = epi(A[M][K] W[N][K]^T + bias): both operands MXFP4 rows, block scales applied by the MFMA, fp32 accumulation, then
- * fw_gemm_bf16's epilogue (bias -> act -> per-column affine g1 / g0 -> + residual -> out_dtype).  C may alias res.
+ * fw_gemm_bf16's epilogue (bias -> act -> per-column affine g1 / g0 -> + residual -> out_dtype).  C may be res: the same rows in the same
+ * type; otherwise the outputs share no byte with any operand (refused).
  * out_dtype FW_DT_MXFP4: the result is rounded to bf16 and quantised along N by the rule above -- the bytes of fw_mxfp4_quant_rows on the
  * bf16 output -- C = codes [M][ldc] (bytes), cs = scales; the input of the next MXFP4 linear without a pass of its own (cs is not used
  * for the other types).  lda, ldw (bytes) < 2^23; M, N < 2^31 - 256.  A row's bits depend on nothing but the row -- except that products of up to 32 rows add
@@ -500,6 +501,8 @@ int fw_linear_mxfp4(const uint16_t* x, int64_t ldx, const uint8_t* W, int64_t ld
  * x / x_out [rows][C] f32 or bf16 (one type), y f32 or bf16; y NULL: no update, h = norm(x) alone (bias, g1, g0, post, x_out unused).
  * g1, g0, scale, shift: [ceil(rows / rows_per_mod)][C] fp32, row r uses vector r / rows_per_mod (one vector for all: rows_per_mod >= rows);
  * bias, post_w, w, b: [C] fp32; NULL = absent.  C <= 8192.
+ * x_out and a bf16 h each may be x or y: the same rows in the same type; otherwise the outputs share no byte with an operand or with each
+ * other (refused).
  * With C = 1024 or 5120, fp32 x, LAYER and no post norm: the bits of fw_residual_add followed by fw_layernorm_mod. */
 #define FW_RNORM_NONE  0
 #define FW_RNORM_LAYER 1

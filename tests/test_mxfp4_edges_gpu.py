@@ -74,3 +74,24 @@ def test_strides_up_to_the_limit(ops, M):
         return far
     assert torch.equal(want, ops.linear(mx, ops.linear_from_mxfp4(spread(wm.q), wm.s, None, K)))
     assert torch.equal(want, ops.linear(MXFP4Rows(spread(mx.q), mx.s, K), ops.linear_from_mxfp4(wm.q, wm.s, None, K)))
+
+
+@pytest.mark.parametrize("M", [5, 40, 300])
+def test_outputs_beside_and_across_operands(ops, M):
+    """Columns of one buffer share nothing; the residual itself is a place for the output; a shifted view of x or of the residual is refused."""
+    N = K = 256
+    wide, lin = rnd(M, 3 * K + 16, seed=1).cuda(), ops.pack_linear_mxfp4(rnd(N, K, seed=2, scale=K ** -0.5), rnd(N, seed=3))
+    x, res, out = wide[:, :K], wide[:, K:2 * K], wide[:, 2 * K:3 * K]
+    want = ops.linear(x, lin, res=res)
+    assert torch.equal(ops.linear(x, lin, res=res, out=out), want)
+    for bad in (dict(out=wide[:, 8:8 + N]), dict(res=res, out=wide[:, K + 8:K + 8 + N]), dict(out=wide[:, K - 1:K - 1 + N])):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            ops.linear(x, lin, **bad)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ops.linear(x[:-1], lin, res=res[:-1], out=res[1:])
+    f32 = torch.zeros(M, N, device="cuda")
+    with pytest.raises(RuntimeError, match="overlaps"):              # the residual's memory in another type
+        ops.linear(x, lin, res=f32, out=f32.view(torch.bfloat16)[:, :N])
+    with pytest.raises(RuntimeError, match="overlaps"):              # the output in the linear's own codes
+        ops.linear(x[:5], lin, out=lin.q[:20].reshape(-1).view(torch.bfloat16).view(5, N))
+    assert torch.equal(ops.linear(x, lin, res=res, out=res), want) and torch.equal(res, want)
