@@ -169,7 +169,7 @@ class MXFP4Rows:
         if q.get_device() != s.get_device():
             raise ValueError(f"MXFP4 codes on {q.device}, scales on {s.device}")
         self._buf, self._q, self._s, self.M, self.K = q, q, s, M, K
-        self.qp, self.sp, self.ldq = q.data_ptr(), s.data_ptr(), q.stride(0)
+        self.qp, self.sp, self.ldq = q.data_ptr(), s.data_ptr(), q.stride(0) if M > 1 else q.shape[1]      # one row's stride says nothing
 
     @classmethod
     def _unwritten(cls, M, K, device):

@@ -118,3 +118,11 @@ def test_a_norm_whose_outputs_meet_an_operand_is_refused(lib):
             assert f(**{v: far(out, -256 * runs)}) != -1
     refused(lib, f(post=1, post_w=far(4)), "overlaps")
     refused(lib, f(w=far(6), b=far(4)), "overlaps")
+
+
+def test_one_row_of_codes_has_any_stride():
+    """A tensor of one row may carry any stride for it; the rows' distance is then their width."""
+    s = torch.zeros(1, 2, 32, 8, dtype=torch.uint8)
+    for q in (torch.zeros(256, 1, dtype=torch.uint8).t(), torch.zeros(1, 256, dtype=torch.uint8).as_strided((1, 256), (7, 1)), torch.zeros(4, 256, dtype=torch.uint8)[1:2]):
+        assert q.shape == (1, 256) and hip_ops.MXFP4Rows(q, s, 300).ldq == 256
+    assert hip_ops.MXFP4Rows(torch.zeros(4, 400, dtype=torch.uint8)[:, :256], s, 300).ldq == 400
