@@ -864,6 +864,9 @@ class HipOps:
         return self._linear_mxfp4(x, lin, **kw)
 
     # ---- the seam between two halves of a block --------------------------------------------------------------------------------------
+    # widths at which residual_norm (LayerNorm, no post norm, fp32 stream) adds a row's statistics in layernorm's order
+    RESIDUAL_NORM_SAME_BITS = (1024, 2048, 5120)
+
     def residual_norm(self, x, y=None, bias=None, g1=None, g0=None, post=None, post_w=None, w=None, b=None, scale=None, shift=None,
                       norm="layer", eps=1e-6, x_out=None, out="bf16", h_out=None):
         """x' = x + [post norm](y + bias) * g1 + g0, written to x_out (default: x, in place); -> h = norm(x') * w + b, * (1 + scale) + shift, as

@@ -240,8 +240,9 @@ class TPFusionEngine(FusionEngine):
     def _reduce_into(self, stream, x_in, lin, bias, g1=None, g0=None, kind="all_reduce", norm=None):
         """stream += (all_reduce(x_in @ lin^T) + bias) * g1 + g0, as a generator: row blocks so that the reduction of block c flies
         behind the GEMM of block c+1 (and behind whatever the interleaved branch enqueues at the yield).
-        norm (layernorm's keywords): what follows is that LayerNorm of the stream and nothing else touches the stream in between -- the
-        update and the norm are one pass (residual_norm: the bits of residual_add, then layernorm), and its rows are returned."""
+        norm (layernorm's keywords): what follows is that LayerNorm of the stream and nothing else touches the stream in between -- at the
+        widths where residual_norm returns the bits of residual_add, then layernorm, the update and the norm are one pass, at others two;
+        the norm's rows are returned."""
         ops, tp = self.ops, self.tp
         M = x_in.shape[0]
         nch = max(1, min(tp.chunks, M // tp.chunk_rows)) if tp.world > 1 else 1
@@ -260,13 +261,14 @@ class TPFusionEngine(FusionEngine):
             part = ops.linear(rows_of(a, b), lin, out_f32=f32)
             pend.append((a, b, tp.all_reduce_async(part, kind)))
         yield
-        h = None if norm is None else ops.empty(M, stream.shape[1])
+        fused = norm is not None and stream.shape[1] in getattr(ops, "RESIDUAL_NORM_SAME_BITS", (stream.shape[1],))
+        h = ops.empty(M, stream.shape[1]) if fused else None
         for a, b, p in pend:
-            if norm is None:
-                ops.residual_add(stream[a:b], p.wait(), bias=bias, g1=g1, g0=g0)
-            else:
+            if fused:
                 ops.residual_norm(stream[a:b], p.wait(), bias=bias, g1=g1, g0=g0, h_out=h[a:b], **norm)
-        return h
+            else:
+                ops.residual_add(stream[a:b], p.wait(), bias=bias, g1=g1, g0=g0)
+        return h if fused or norm is None else ops.layernorm(stream, **norm)
 
     def _stats(self, *slices):
         """Sum of squares over the FULL width of each row for several (rows, local-columns) slices: one fused all-reduce."""

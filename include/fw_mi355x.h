@@ -503,7 +503,7 @@ int fw_linear_mxfp4(const uint16_t* x, int64_t ldx, const uint8_t* W, int64_t ld
  * bias, post_w, w, b: [C] fp32; NULL = absent.  C <= 8192.
  * x_out and a bf16 h each may be x or y: the same rows in the same type; otherwise the outputs share no byte with an operand or with each
  * other (refused).
- * With C = 1024 or 5120, fp32 x, LAYER and no post norm: the bits of fw_residual_add followed by fw_layernorm_mod. */
+ * With C = 1024, 2048 or 5120, fp32 x, LAYER and no post norm: the bits of fw_residual_add followed by fw_layernorm_mod. */
 #define FW_RNORM_NONE  0
 #define FW_RNORM_LAYER 1
 #define FW_RNORM_RMS   2

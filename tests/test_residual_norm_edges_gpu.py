@@ -62,3 +62,26 @@ def test_outputs_beside_and_across_inputs(ops):
             ops.residual_norm(x, y, **kw)
     with pytest.raises(RuntimeError, match="overlaps"):
         ops.residual_norm(x[:-1], y[1:], x_out=x[1:])
+
+
+@pytest.mark.parametrize("C", [512, 640, 1024, 1280, 1536, 2048, 4096, 5120])
+def test_a_reduced_update_and_its_norm_at_any_width(ops, C):
+    """The tensor-parallel engine's update with a norm behind it returns the bits of residual_add, then layernorm, at every width."""
+    from fantasy_world_amd.tensor_parallel import TensorShard, TPFusionEngine, _drain
+    rows = 8192
+    eng = TPFusionEngine.__new__(TPFusionEngine)
+    eng.ops, eng.tp = ops, TensorShard(0, 1, chunks=2, chunk_rows=64)
+    a, y = rnd(rows, C, seed=1, scale=2.0) + 0.3, rnd(rows, 64, seed=2, dtype=torch.bfloat16)
+    lin, bias, g1, w, b = ops.pack_linear(rnd(C, 64, seed=3).cpu(), None), rnd(C, seed=4), rnd(C, seed=5), rnd(C, seed=6), rnd(C, seed=7)
+    norm = dict(w=w, b=b, eps=1e-6)
+    x, box = a.clone(), {}
+
+    def fused():
+        box["rows"] = yield from eng._reduce_into(x, y, lin, bias, g1=g1, norm=norm)
+    _drain(fused())
+    _drain(eng._reduce_into(a, y, lin, bias, g1=g1))
+    assert torch.equal(x, a) and torch.equal(box["rows"], ops.layernorm(a, **norm))
+    if C in ops.RESIDUAL_NORM_SAME_BITS:
+        part = ops.linear(y, lin, out_f32=eng.tp.reduce_dtype == torch.float32)
+        again = rnd(rows, C, seed=1, scale=2.0) + 0.3
+        assert torch.equal(ops.residual_norm(again, part, bias=bias, g1=g1, **norm), box["rows"]) and torch.equal(again, a)
