@@ -502,9 +502,10 @@ def init_from_env(backend=None):
     return topo.shard, topo.rank, topo.world, topo.local
 
 
-GOLDEN_TOL = {"bf16": 8e-3, "fp8": 8e-2, "mxfp4": 0.35}     # rel-L2 of noise_pred against the fp32 reference golden; fp8: e4m3's own price (measured
+GOLDEN_TOL = {"bf16": 8e-3, "fp8": 8e-2, "mxfp4": 0.18}      # rel-L2 of noise_pred against the fp32 reference golden; fp8: e4m3's own price (measured
                                              # 4.7e-2 on one GPU, tests/golden/parity_bounds_gpu.json `fp8/wan21_cfg1...`, fp8 attention included);
-                                             # mxfp4: the relative error of an e2m1 x e2m1 linear is 0.16 against e4m3's 0.037, 4.4 times fp8's
+                                             # mxfp4: 0.134 to 0.146 measured over the cases; wrong scales in an eighth of one rank's weights make
+                                             # it 0.238 (two ranks, wan21_l3_f2_12x8)
 
 
 def golden_self_check(topo, ops, case="wan21_cfg1_l2_f9_64x64", tol=None, golden_dir=None, precision="bf16", fp8_attention=False):
