@@ -56,16 +56,25 @@ __device__ __forceinline__ void mx_tile(const MxArgs& p, int& tm, int& tn) {
     tn = in_g / gsz;
 }
 
-// GELU with erf by Abramowitz & Stegun 7.1.26 (|error of erf| <= 1.5e-7), in its complementary form: no cancellation for negative values.
-// erff in its place costs 14 us per 128 x 256 tile.  Past 8 the value is x itself in fp32 (1 - Phi(8) = 6e-16), infinity included, where the
-// difference below would be inf - inf * 0; at -infinity the formula is -inf * 0, a NaN, here as there.
+// GELU with erf:  x Phi(x) = max(x, 0) - |x| / 2 * erfc(|x| / sqrt 2),  no cancellation on either side.  log2 erfc(z / sqrt 2) is smooth and 0 at 0:
+// a polynomial of degree 10 without constant term, fitted to 64-bit values on [0, 6] by least squares reweighted towards the smallest
+// largest error, each point weighted by erfc itself down to 1e-3.  Error of erfc 6e-9 + fp32 rounding: 3.3e-8 of N(0, 0.3^2) and 2.8e-8 of N(0, 1) in the
+// 2-norm, where 0.5 x (1 + erf) in fp32 is 4e-8 off.  Past 6 it falls on (the leading term is negative).  erff in its place costs 14 us per
+// 128 x 256 tile.  Past 8 the value is x itself in fp32 (1 - Phi(8) = 6e-16), infinity included, where the difference below would be
+// inf - inf * 0; at -infinity the formula is -inf * 0, a NaN, here as there.
 __device__ __forceinline__ float mx_gelu_erf(float x) {
-    const float z = fabsf(x) * 0.7071067811865476f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
-    float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-    q = __builtin_fmaf(q, t, 1.421413741f);
-    q = __builtin_fmaf(q, t, -0.284496736f);
-    q = __builtin_fmaf(q, t, 0.254829592f);
-    const float v = fmaxf(x, 0.f) - 0.5f * fabsf(x) * (q * t * __expf(-z * z));
+    const float z = fabsf(x);
+    float q = -2.8891838e-8f;
+    q = __builtin_fmaf(q, z, 8.6283444e-7f);
+    q = __builtin_fmaf(q, z, -1.1020638e-5f);
+    q = __builtin_fmaf(q, z, 7.6711956e-5f);
+    q = __builtin_fmaf(q, z, -2.7991601e-4f);
+    q = __builtin_fmaf(q, z, -1.5661665e-6f);
+    q = __builtin_fmaf(q, z, 6.9519272e-3f);
+    q = __builtin_fmaf(q, z, -5.2446816e-2f);
+    q = __builtin_fmaf(q, z, -4.5921841e-1f);
+    q = __builtin_fmaf(q, z, -1.1511044f);
+    const float v = __builtin_fmaf(-0.5f * z, __builtin_amdgcn_exp2f(q * z), fmaxf(x, 0.f));
     return x > 8.f ? x : v;
 }
 template <int ACT>

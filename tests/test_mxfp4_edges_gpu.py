@@ -95,3 +95,20 @@ def test_outputs_beside_and_across_operands(ops, M):
     with pytest.raises(RuntimeError, match="overlaps"):              # the output in the linear's own codes
         ops.linear(x[:5], lin, out=lin.q[:20].reshape(-1).view(torch.bfloat16).view(5, N))
     assert torch.equal(ops.linear(x, lin, res=res, out=res), want) and torch.equal(res, want)
+
+
+@pytest.mark.parametrize("M,N", [(3, 4096), (20, 4096), (300, 4096), (4352, 4096)])
+@pytest.mark.parametrize("spread", [0.3, 1.0, 3.0])
+def test_gelu_keeps_the_digits_of_fp32(ops, M, N, spread):
+    """fp32 output of the erf GELU on arguments that carry no error of their own (a zero product, the bias is the argument).
+    Each of |x| / 2, the tail's exponent, its power of two and the result rounds once or is good to a unit in the last place: 2^-24 of values that
+    are no larger than |x| / 2 each, 1e-5 of the tail where it is below 1e-3.  In the 2-norm over random arguments the result is within 5e-8,
+    which 0.5 x (1 + erf) in fp32 just reaches (4e-8)."""
+    b = rnd(N, seed=3, scale=spread, dtype=torch.float32)
+    lin = ops.pack_linear_mxfp4(rnd(N, 1024, seed=2), b)
+    got = ops.linear(torch.zeros(M, 1024, dtype=torch.bfloat16, device="cuda"), lin, act="gelu_erf", out_f32=True)
+    want = act64(b.double(), "gelu_erf").cuda()
+    assert torch.equal(got, got[:1].expand_as(got))
+    off = (got[0].double() - want).abs()
+    assert (off <= 4 * 2.0 ** -24 * want.abs().clamp(min=0) + 4 * 2.0 ** -24 * 0.5 * b.double().abs().cuda()).all()
+    assert (got[0].double() - want).norm() / want.norm() < 5e-8
