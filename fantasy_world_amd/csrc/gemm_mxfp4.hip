@@ -258,10 +258,8 @@ __device__ __forceinline__ void mx_finish(const MxArgs& p, char* reg, const Acc&
 
 // ---------------------------------------------------------------------------------------------------------------
 // BM x BN tiles, K slabs of 256 values in a ring of ST stages: four waves multiply (wave tile 32 x 64 at 64 x 128, 64 x 64 at 64 x 256, 128 x 64
-// at 128 x 256), four others do nothing but request codes and scale bytes by LDS-DMA, ST - 1 slabs ahead; one barrier a slab.  A slab past
-// the end is requested out of the descriptors' range (zeros into a stage that nobody reads any more), so the loaders' counted wait is the
-// same number in every iteration.  The descriptors end with the last byte of their last row: 255 strides below 2^23 and 2^23 bytes make
-// less than 2^31, and the lane offset of a request past the end starts there.
+// at 128 x 256), four others do nothing but request codes and scale bytes by LDS-DMA, ST - 1 slabs ahead; one barrier a slab.  Nothing is
+// requested past the last slab: the wait for it is the one for everything.
 // Why loaders of their own: a wave that requests its slab is held until the CU's path from L2 (64 bytes a clock) has taken the request, and
 // with one multiplying wave on a SIMD nobody multiplies meanwhile -- 257 x 5120 x 13824 took 39 us with four waves doing both, at two stages
 // as at four, and takes 21.7 with loaders.  What bounds it now is LDS (the waves' fragment reads and the DMA's writes: 574, 840 and 1150
@@ -283,7 +281,6 @@ __global__ __launch_bounds__(512, ST * (BM + BN) * 136 <= 80 * 1024 ? 4 : 2) voi
     int tm, tn;
     mx_tile(p, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
-    constexpr unsigned PAST = 0x80000000u;
     const auto ars = mx_rows_rsrc(p.A + (int64_t)m0 * p.lda, min(p.M - m0, BM), p.lda, p.slabs);
     const auto wrs = mx_rows_rsrc(p.W + (int64_t)n0 * p.ldw, min(p.N - n0, BN), p.ldw, p.slabs);
     const int sstride = __builtin_amdgcn_readfirstlane(p.slabs * 256);
@@ -295,17 +292,16 @@ __global__ __launch_bounds__(512, ST * (BM + BN) * 136 <= 80 * 1024 ? 4 : 2) voi
     const int astep = __builtin_amdgcn_readfirstlane((int)p.lda * 8), wstep = __builtin_amdgcn_readfirstlane((int)p.ldw * 8);
     auto issue = [&](char* st, int kt) __attribute__((always_inline)) {
         const int k0 = kt * 128, s0 = kt * 256;
-        const int live = kt < p.slabs ? -1 : 0, past = (int)PAST & ~live;
 #pragma unroll
-        for (int j = 0; j < APC; ++j) FWX_BLDS16(ars, va[j & 1] | past, (k0 + (wave * APC + j) * astep) & live, st + (wave * APC + j) * 1024);
+        for (int j = 0; j < APC; ++j) FWX_BLDS16(ars, va[j & 1], k0 + (wave * APC + j) * astep, st + (wave * APC + j) * 1024);
 #pragma unroll
-        for (int j = 0; j < WPC; ++j) FWX_BLDS16(wrs, vw[j & 1] | past, (k0 + (wave * WPC + j) * wstep) & live, st + BM * 128 + (wave * WPC + j) * 1024);
+        for (int j = 0; j < WPC; ++j) FWX_BLDS16(wrs, vw[j & 1], k0 + (wave * WPC + j) * wstep, st + BM * 128 + (wave * WPC + j) * 1024);
 #pragma unroll
         for (int j = 0; j < SPC; ++j) {
             const int g = min(wave + 4 * j, RB - 1);
             char* d = st + (BM + BN) * 128 + g * 256;
-            if (g < BM / 32) __builtin_amdgcn_raw_ptr_buffer_load_lds(sars, FW_LDS_PTR(d), 4, lane * 4 | past, (s0 + g * sstride) & live, 0, 0);
-            else __builtin_amdgcn_raw_ptr_buffer_load_lds(swrs, FW_LDS_PTR(d), 4, lane * 4 | past, (s0 + (g - BM / 32) * sstride) & live, 0, 0);
+            if (g < BM / 32) __builtin_amdgcn_raw_ptr_buffer_load_lds(sars, FW_LDS_PTR(d), 4, lane * 4, s0 + g * sstride, 0, 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(swrs, FW_LDS_PTR(d), 4, lane * 4, s0 + (g - BM / 32) * sstride, 0, 0);
         }
     };
     const int swz = (fi >> 1) & 7;
@@ -313,16 +309,17 @@ __global__ __launch_bounds__(512, ST * (BM + BN) * 136 <= 80 * 1024 ? 4 : 2) voi
     const int s_a = (BM + BN) * 128 + wm * WM * 256 + fi * 8 + hi * 4, s_w = (BM + BN) * 128 + (BM / 32 + wn * 2) * 256 + fi * 8 + hi * 4;
 
     if (wave8 >= 4) {
-#pragma unroll
-        for (int i = 0; i < ST - 1; ++i) issue(smem + i * STAGE, i);
-        int nxt = ST - 1;                                 // stage of slab kt + ST - 1: that of kt - 1
+        static_assert(ST == 3, "a wait leaves the one slab after its own in flight");
+        issue(smem, 0);
+        if (p.slabs > 1) issue(smem + STAGE, 1);
+        int nxt = 2;                                      // stage of slab kt + 2: that of kt - 1
         for (int kt = 0; kt < p.slabs; ++kt) {
-            mx_wait_vm<(ST - 2) * (APC + WPC + SPC)>();   // this wave's pieces of slab kt ...
+            if (kt + 1 < p.slabs) mx_wait_vm<APC + WPC + SPC>();      // this wave's pieces of slab kt ...
+            else mx_wait_vm<0>();
             FWX_BARRIER();                                // ... and every loader's; the others have read slab kt - 1
-            issue(smem + nxt * STAGE, kt + ST - 1);
-            nxt = nxt + 1 == ST ? 0 : nxt + 1;
+            if (kt + 2 < p.slabs) issue(smem + nxt * STAGE, kt + 2);
+            nxt = nxt == 2 ? 0 : nxt + 1;
         }
-        mx_wait_vm<0>();                                  // the requests past the end
         FWX_BARRIER();
         return;
     }
