@@ -80,7 +80,7 @@ __device__ __forceinline__ float mx_gelu_erf(float x) {
 template <int ACT>
 __device__ __forceinline__ float mx_act(float v) {
     // a block with a NaN makes its products NaN, and a ReLU keeps them: (v > 0 ? v : 0) would answer 0
-    if (ACT == FW_ACT_RELU) return v <= 0.f ? 0.f : v;
+    if (ACT == FW_ACT_RELU) return __builtin_elementwise_maximum(v, 0.f);
     return ACT == FW_ACT_GELU_ERF ? mx_gelu_erf(v) : fw_apply_act(v, ACT);
 }
 
