@@ -3,7 +3,8 @@
 // x' goes back to the stream, h leaves in bf16 or as MXFP4 rows for the linear that follows.  Run apart (fw_residual_add, then
 // fw_layernorm_mod, then fw_mxfp4_quant_rows) the stream is read twice and h written and read once more.  Bound by HBM.
 // One wave per row, the row in registers (VPL float4 a lane, C <= 256 VPL), statistics by wave shuffles in row_norm.h's pinned order:
-// with LayerNorm, no post norm and C = 256 VPL the results are the bits of fw_residual_add followed by fw_layernorm_mod.
+// with LayerNorm, no post norm and 1024, 2048 or 5120 columns (one wave a row there too) the results are the bits of fw_residual_add followed
+// by fw_layernorm_mod.
 #include "mxfp4.h"
 #include "row_norm.h"
 

@@ -465,8 +465,8 @@ int fw_gemm_fp8(const uint8_t* A, int64_t lda, const uint8_t* W, int64_t ldw, co
  *   aligned: s[r / 32][k / 256][r % 32][k / 32 % 8].  Scale bytes of the padding past K are not 0xff; those of rows past M are not read as values.
  * ------------------------------------------------------------------------------------------------------------- */
 
-/* x [M][K] (bf16 or f32, ldx elements, any K and alignment of the element type) -> MXFP4 rows.  8 values per access where K % 8 == 0 and
- * the rows are 16-byte aligned, one at a time otherwise. */
+/* x [M][K] (bf16 or f32, ldx elements, any K and alignment of the element type) -> MXFP4 rows.  8 values per access at any alignment, the
+ * last K % 8 of a row singly. */
 int fw_mxfp4_quant_rows(const void* x, int64_t ldx, int x_dtype, uint8_t* q, int64_t ldq, uint8_t* s, int M, int K, void* stream);
 
 /* MXFP4 rows -> y [M][K] (bf16 or f32; exact in both). */
